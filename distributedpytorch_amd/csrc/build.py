@@ -34,6 +34,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffast-math",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-fno-gpu-rdc", "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
+# Sources compiled without -ffast-math: their inputs may hold infinities and NaN (masked places, overflowed maps), which
+# fast-math lets the compiler assume away, and their sums keep the order that is written.
+STRICT_MATH = ("cross_attention.hip", "dropout.hip", "group_norm.hip")
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fopenmp", "-Wall"]
 HIP_LIB = os.path.join(HERE, "libdpamd_hip.so")
 HOST_LIB = os.path.join(HERE, "libdpamd_host.so")
@@ -57,9 +60,15 @@ def hip_sources():
     return sorted(glob.glob(os.path.join(HERE, "*.hip")))
 
 
+def hip_flags(src: str):
+    if os.path.basename(src) in STRICT_MATH:
+        return [f for f in HIP_FLAGS if f != "-ffast-math"]
+    return HIP_FLAGS
+
+
 def source_hash() -> str:
     """Hash of everything ``libdpamd_hip.so`` is made from (sources, headers, flags)."""
-    return _sha(hip_sources() + _headers(), " ".join(HIP_FLAGS))[:32]
+    return _sha(hip_sources() + _headers(), " ".join([*HIP_FLAGS, *STRICT_MATH]))[:32]
 
 
 def host_source_hash() -> str:
@@ -131,14 +140,14 @@ def build_all(force: bool = False, verbose: bool = False, save_asm: bool = False
 def _build_all_locked(force: bool, verbose: bool, save_asm: bool) -> bool:
     headers = _headers()
     hip_srcs = hip_sources()
-    flags = " ".join(HIP_FLAGS)
     objs, jobs, stamps = [], [], []
     for src in hip_srcs:
         obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
         objs.append(obj)
-        want = _sha([src] + headers, flags)
+        flags = hip_flags(src)
+        want = _sha([src] + headers, " ".join(flags))
         if force or not os.path.isfile(obj) or _read(obj + ".hash") != want:
-            cmd = [HIPCC, *HIP_FLAGS, "-c", src, "-o", obj]
+            cmd = [HIPCC, *flags, "-c", src, "-o", obj]
             if save_asm:
                 cmd += ["-save-temps=obj"]
             jobs.append(cmd)

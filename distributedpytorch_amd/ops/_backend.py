@@ -13,6 +13,7 @@ Policy
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import sys
@@ -194,6 +195,13 @@ def lib_current() -> bool:
 def stream_ptr() -> ctypes.c_void_p:
     """Current HIP stream as a raw ``hipStream_t`` for the C launchers."""
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def on_device(t: torch.Tensor):
+    """Context for a launch on ``t``'s own GPU (its current stream, its allocations), whichever GPU is current."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
