@@ -1,0 +1,742 @@
+// Attention of one sequence's queries over another's keys and values, forward and backward.
+//
+//   S = scale q k^T over the keys that take part,  P = softmax(S),  o = P v;   a row without a key gives 0
+//   backward, delta = rowsum(do o):   dv = P^T do    dS = P (do v^T - delta) scale    dq = dS k    dk = dS^T q
+//
+// Heads: q has Hq = Hk * share of them; share neighbouring query heads read one key / value head.  The kernels see, per
+// (image, key head), R = Lq * share ROWS (row r: position r / share, head r % share), so shared heads read keys once and
+// their gradients add up in the row sum.
+//
+// Everything runs on v_mfma_f32_32x32x16 with fp32 accumulators and never writes a score to memory: the first product
+// leaves rows (or keys) on the lanes and keys (or rows) on the accumulator registers, which, packed in pairs, ARE the
+// second operand of the product that contracts over them; the first operand of that product comes out of the row-major
+// LDS tile through transposing reads.
+//
+//   xa_fwd    128 rows a workgroup (32 a wave), keys in blocks of 64 through LDS, running maximum and sum; with few rows
+//             the keys are split over workgroups and xa_join puts the parts together
+//   xa_delta  delta per row
+//   xa_dkv    128 keys a workgroup (32 a wave, their k and v in registers), rows in blocks of 32 through LDS
+//   xa_dq     128 rows a workgroup, keys in blocks of 64
+//   xa_sum    joins the fp32 parts of dq, or of dk and dv, where a long axis was split; one order, no atomics
+//
+// P and dS are rounded to the tensors' type before their second product (its operands are 16 bits wide); sums, statistics
+// and gradients' accumulators stay in 32 bits.  Masked keys: their scores are replaced, and their k and v rows are staged
+// as zeros, so whatever they hold (infinities, NaN) takes no part.
+#include "common.h"
+
+namespace {
+
+typedef _Float16 f16;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+struct Bf {
+    typedef bf16_raw raw;
+    static __device__ __forceinline__ f32x16 mfma(const uint4& a, const uint4& b, const f32x16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ unsigned pair(float lo, float hi) { return pack2(lo, hi); }
+    static __device__ __forceinline__ void unpair(unsigned u, float& lo, float& hi) {
+        lo = __uint_as_float(u << 16); hi = __uint_as_float(u & 0xffff0000u);
+    }
+};
+
+struct Hf {
+    typedef f16 raw;
+    static __device__ __forceinline__ f32x16 mfma(const uint4& a, const uint4& b, const f32x16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ unsigned pair(float lo, float hi) {
+        const f16 a = (f16)lo, b = (f16)hi;
+        return (unsigned)__builtin_bit_cast(unsigned short, a) | ((unsigned)__builtin_bit_cast(unsigned short, b) << 16);
+    }
+    static __device__ __forceinline__ void unpair(unsigned u, float& lo, float& hi) {
+        lo = (float)__builtin_bit_cast(f16, (unsigned short)u); hi = (float)__builtin_bit_cast(f16, (unsigned short)(u >> 16));
+    }
+};
+
+constexpr int kRows = 128;       // rows (forward, dq) or keys (dkv) of a workgroup: 4 waves x 32
+constexpr int kKeys = 64;        // keys of an LDS block (forward, dq)
+constexpr int kStep = 32;        // rows of an LDS block (dkv)
+constexpr float kInf = __builtin_huge_valf();
+
+// strides in elements: image, position, head (elements of a head are adjacent)
+struct View { long b, l, h; };
+
+struct Att {
+    const void *q, *k, *v, *o, *dout;
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;              // [B, Hk, R]: log2 of the row's sum of exponentials (+inf: no key), rowsum(do o)
+    const int* lens;                 // [B] keys of each image, or null
+    const unsigned char* mask;       // [B, Lk], nonzero = takes part, or null
+    long mask_ld;
+    View vq, vk, vv, vd;             // of q, k, v and dout (o, dq, dk, dv are dense)
+    int B, Lq, Lk, Hk, share, D;
+    int R;                           // Lq share
+    float scale, c;                  // c = scale log2(e)
+    int splits;                      // parts of the split axis
+    float* part;                     // their fp32 partial results
+};
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// Consecutive workgroups go round the 8 XCDs: give each XCD one contiguous range of the work, so that the workgroups
+// that read the same keys share an L2.
+__device__ __forceinline__ long xcd_order(long id, long total) {
+    const long x = id & 7, i = id >> 3, q = total >> 3, r = total & 7;
+    return x * q + (x < r ? x : r) + i;
+}
+
+// eight columns of this lane's column pair, rows r0..r0+3 and r1..r1+3 of a row-major tile (two transposing reads)
+__device__ __forceinline__ uint4 tr_pair(const unsigned char* a0, const unsigned char* a1) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a0);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a1);
+    return __builtin_bit_cast(uint4, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// accumulator registers 8 s .. 8 s + 7 as an operand of 16 contracted entries: lane half h holds entries
+// 16 s + 4 h + {0..3} and 16 s + 8 + 4 h + {0..3} of the 32
+template <typename E> __device__ __forceinline__ uint4 pack_acc(const f32x16& a, int s) {
+    uint4 u;
+    u.x = E::pair(a[8 * s + 0], a[8 * s + 1]); u.y = E::pair(a[8 * s + 2], a[8 * s + 3]);
+    u.z = E::pair(a[8 * s + 4], a[8 * s + 5]); u.w = E::pair(a[8 * s + 6], a[8 * s + 7]);
+    return u;
+}
+
+// entry of the 32 that accumulator register r of lane half h belongs to
+__device__ __forceinline__ int entry(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// 64-bit set of the keys of block kb that take part; every wave of the workgroup gets the same set
+__device__ __forceinline__ unsigned long long key_set(const Att& p, int b, int len, int kb) {
+    const int key = kb * 64 + (int)(threadIdx.x & 63);
+    bool on = key < len;
+    if (on && p.mask) on = p.mask[(long)b * p.mask_ld + key] != 0;
+    return __ballot(on);
+}
+
+__device__ __forceinline__ int key_count(const Att& p, int b) {
+    if (!p.lens) return p.Lk;
+    const int n = p.lens[b];
+    return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
+}
+
+// offset of row r of key head hk in a tensor of rows
+__device__ __forceinline__ int position(const Att& p, int r) { return p.share == 1 ? r : (int)((unsigned)r / (unsigned)p.share); }
+
+__device__ __forceinline__ long row_at(const Att& p, const View& v, int b, int hk, int r) {
+    const int l = position(p, r);
+    return b * v.b + l * v.l + (hk * p.share + (r - l * p.share)) * v.h;
+}
+
+// the same in a dense [B, Lq, Hq, D] tensor
+__device__ __forceinline__ long dense_row(const Att& p, int b, int hk, int r) {
+    const int l = position(p, r);
+    return (((long)b * p.Lq + l) * (p.Hk * p.share) + hk * p.share + (r - l * p.share)) * p.D;
+}
+
+// one 16-byte piece of NROWS x DP tile rows per thread and step; `ok` decides whether a row is read or zero
+template <int DP, int NROWS> struct Stage {
+    static constexpr int kPieces = (NROWS * DP / 8 + 255) / 256;   // 16-byte pieces of a thread
+    static constexpr int kLd = DP * 2 + 16;                        // LDS bytes of a row: 16 of padding spread the banks
+    static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * 256) / (DP / 8); }
+    static __device__ __forceinline__ int col(int i) { return ((int)threadIdx.x + i * 256) % (DP / 8) * 8; }
+    static __device__ __forceinline__ void put(unsigned char* tile, const uint4 (&u)[kPieces]) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            if (NROWS * DP / 8 % 256 == 0 || row(i) < NROWS) *reinterpret_cast<uint4*>(tile + row(i) * kLd + col(i) * 2) = u[i];
+    }
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ void fetch_keys(const Att& p, const void* base, const View& v, int b, int hk, int kb,
+                                           unsigned long long set, uint4 (&u)[Stage<DP, kKeys>::kPieces]) {
+    typedef Stage<DP, kKeys> S;
+    const T* t = (const T*)base + b * v.b + hk * v.h;
+#pragma unroll
+    for (int i = 0; i < S::kPieces; ++i) {
+        u[i] = make_uint4(0, 0, 0, 0);
+        if (S::row(i) < kKeys && (set >> S::row(i) & 1) && S::col(i) < p.D)
+            u[i] = *reinterpret_cast<const uint4*>(t + ((long)kb * kKeys + S::row(i)) * v.l + S::col(i));
+    }
+}
+
+// this lane's row as the second operand (contracted over the head's width): DP / 16 pieces of 8 elements
+template <typename T, int DP>
+__device__ __forceinline__ void row_operand(const Att& p, const void* base, const View& v, int b, int hk, int r, bool on,
+                                            uint4 (&f)[DP / 16]) {
+    const int h = (threadIdx.x & 63) >> 5;
+    const T* t = (const T*)base + (on ? row_at(p, v, b, hk, r) : 0);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d = ks * 16 + h * 8;
+        f[ks] = make_uint4(0, 0, 0, 0);
+        if (on && d < p.D) f[ks] = *reinterpret_cast<const uint4*>(t + d);
+    }
+}
+
+struct Work { int b, hk, tile, split; };
+
+// work item: tiles fastest, then splits, then (image, key head)
+__device__ __forceinline__ Work work_of(const Att& p, int tiles) {
+    const long id = xcd_order(blockIdx.x, gridDim.x);
+    Work w;
+    w.tile = (int)(id % tiles);
+    const long t = id / tiles;
+    w.split = (int)(t % p.splits);
+    const long bh = t / p.splits;
+    w.hk = (int)(bh % p.Hk);
+    w.b = (int)(bh / p.Hk);
+    return w;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void xa_fwd_kernel(Att p, int tiles) {
+    typedef typename E::raw T;
+    typedef Stage<DP, kKeys> S;
+    __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
+    __shared__ __attribute__((aligned(16))) unsigned char Vs[2][kKeys * S::kLd];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+    const Work w = work_of(p, tiles);
+    const int r = w.tile * kRows + wave * 32 + l31;
+    const bool row_on = r < p.R, wave_on = w.tile * kRows + wave * 32 < p.R;
+    const int len = key_count(p, w.b);
+    const int nkb = (len + kKeys - 1) / kKeys;
+    const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
+
+    uint4 qf[DP / 16];
+    row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r, row_on, qf);
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
+    float m = -kInf, l = 0.f;
+
+    uint4 kreg[S::kPieces], vreg[S::kPieces];
+    unsigned long long set = 0, next = 0;
+    if (kb0 < kb1) {
+        next = key_set(p, w.b, len, kb0);
+        fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb0, next, kreg);
+        fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb0, next, vreg);
+    }
+    for (int kb = kb0; kb < kb1; ++kb) {
+        unsigned char *kt = Ks[kb & 1], *vt = Vs[kb & 1];
+        S::put(kt, kreg);
+        S::put(vt, vreg);
+        set = next;
+        __syncthreads();                     // (two buffers: the block before last is read no more)
+        if (kb + 1 < kb1) {
+            next = key_set(p, w.b, len, kb + 1);
+            fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb + 1, next, kreg);
+            fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb + 1, next, vreg);
+        }
+        if (!wave_on || set == 0) continue;
+        // S^T: keys on the registers, this lane's row
+        f32x16 st[2] = {zero16(), zero16()};
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint4 kf = *reinterpret_cast<const uint4*>(kt + (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2);
+                st[t] = E::mfma(kf, qf[ks], st[t]);
+            }
+        if (set != ~0ull) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(bits >> entry(i, 0) & 1)) st[t][i] = -kInf;
+            }
+        }
+        float mx = st[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) mx = fmaxf(mx, st[i >> 4][i & 15]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mnew = fmaxf(m, mx);
+        const float mc = mnew == -kInf ? 0.f : mnew * p.c;
+        if (__any(mnew != m)) {
+            const float alpha = __builtin_amdgcn_exp2f(fmaf(m, p.c, -mc));       // (m = -inf: 0)
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+            m = mnew;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(st[t][i], p.c, -mc));
+                st[t][i] = e;
+                l += e;
+            }
+        // O^T += V^T P^T
+        const unsigned char* vb = vt + (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const uint4 pf = pack_acc<E>(st[s >> 1], s & 1);
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t) {
+                const unsigned char* a = vb + (16 * s) * S::kLd + t * 64;
+                acc[t] = E::mfma(tr_pair(a, a + 8 * S::kLd), pf, acc[t]);
+            }
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (!row_on) return;
+    const long bh = (long)w.b * p.Hk + w.hk;
+    if (p.splits > 1) {
+        float* o = p.part + ((bh * p.splits + w.split) * p.R + r) * (DP + 2);
+        if (h == 0) { o[DP] = m; o[DP + 1] = l; }
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t * 32 + entry(i, h)] = acc[t][i];
+        return;
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    if (h == 0 && p.lse) p.lse[bh * p.R + r] = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : kInf;
+    T* o = (T*)p.out + dense_row(p, w.b, w.hk, r);
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = t * 32 + 8 * g + 4 * h;
+            if (d < p.D) {
+                uint2 u;
+                u.x = E::pair(acc[t][4 * g] * inv, acc[t][4 * g + 1] * inv);
+                u.y = E::pair(acc[t][4 * g + 2] * inv, acc[t][4 * g + 3] * inv);
+                *reinterpret_cast<uint2*>(o + d) = u;
+            }
+        }
+}
+
+// joins the splits of one row: a wave per row
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
+    typedef typename E::raw T;
+    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (id >= rows) return;
+    const long bh = id / p.R;
+    const int r = (int)(id - bh * p.R);
+    const float* base = p.part + (bh * p.splits * p.R + r) * (DP + 2);
+    const long step = (long)p.R * (DP + 2);
+    float m = -kInf;
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, base[s * step + DP]);
+    const float mc = m == -kInf ? 0.f : m * p.c;
+    float l = 0.f, a0 = 0.f, a1 = 0.f;
+    const int d = lane * 2;
+    for (int s = 0; s < p.splits; ++s) {
+        const float* o = base + s * step;
+        const float f = __builtin_amdgcn_exp2f(fmaf(o[DP], p.c, -mc));
+        l = fmaf(o[DP + 1], f, l);
+        if (d < p.D) { a0 = fmaf(o[d], f, a0); a1 = fmaf(o[d + 1], f, a1); }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    if (lane == 0 && p.lse) p.lse[id] = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : kInf;
+    if (d < p.D) {
+        const int b = (int)(bh / p.Hk), hk = (int)(bh % p.Hk);
+        T* o = (T*)p.out + dense_row(p, b, hk, r);
+        *reinterpret_cast<unsigned*>(o + d) = E::pair(a0 * inv, a1 * inv);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// delta[row] = sum_d do o: 16 lanes a row
+template <typename E>
+__global__ __launch_bounds__(256) void xa_delta_kernel(Att p, long rows) {
+    typedef typename E::raw T;
+    const long id = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int g = threadIdx.x & 15;
+    if (id >= rows) return;
+    const long bh = id / p.R;
+    const int r = (int)(id - bh * p.R);
+    const int b = (int)(bh / p.Hk), hk = (int)(bh % p.Hk);
+    const T* o = (const T*)p.o + dense_row(p, b, hk, r);
+    const T* d = (const T*)p.dout + row_at(p, p.vd, b, hk, r);
+    float s = 0.f;
+    if (g * 8 < p.D) {
+        const uint4 a = *reinterpret_cast<const uint4*>(o + g * 8), c = *reinterpret_cast<const uint4*>(d + g * 8);
+        const unsigned av[4] = {a.x, a.y, a.z, a.w}, cv[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a0, a1, c0, c1;
+            E::unpair(av[i], a0, a1);
+            E::unpair(cv[i], c0, c1);
+            s = fmaf(a0, c0, fmaf(a1, c1, s));
+        }
+    }
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
+    if (g == 0) p.delta[id] = s;
+}
+
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void xa_dkv_kernel(Att p, int tiles) {
+    typedef typename E::raw T;
+    typedef Stage<DP, kStep> S;
+    __shared__ __attribute__((aligned(16))) unsigned char Qs[2][kStep * S::kLd];
+    __shared__ __attribute__((aligned(16))) unsigned char Ds[2][kStep * S::kLd];
+    __shared__ __attribute__((aligned(16))) float Ls[2][2][kStep];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+    const Work w = work_of(p, tiles);
+    const int key = w.tile * kRows + wave * 32 + l31;
+    const int len = key_count(p, w.b);
+    bool on = key < len;
+    if (on && p.mask) on = p.mask[(long)w.b * p.mask_ld + key] != 0;
+    const bool wave_on = __any(on);
+    const long bh = (long)w.b * p.Hk + w.hk;
+    const int nst = (p.R + kStep - 1) / kStep;
+    const int st0 = (int)((long)nst * w.split / p.splits);
+    const int st1 = w.tile * kRows < len ? (int)((long)nst * (w.split + 1) / p.splits) : st0;
+
+    uint4 kf[DP / 16], vf[DP / 16];
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d = ks * 16 + h * 8;
+        kf[ks] = vf[ks] = make_uint4(0, 0, 0, 0);
+        if (on && d < p.D) {
+            kf[ks] = *reinterpret_cast<const uint4*>((const T*)p.k + w.b * p.vk.b + w.hk * p.vk.h + key * p.vk.l + d);
+            vf[ks] = *reinterpret_cast<const uint4*>((const T*)p.v + w.b * p.vv.b + w.hk * p.vv.h + key * p.vv.l + d);
+        }
+    }
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
+
+    uint4 qreg[S::kPieces], dreg[S::kPieces];
+    float lreg = 0.f;
+    auto fetch = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) {
+            const int r = st * kStep + S::row(i);
+            qreg[i] = dreg[i] = make_uint4(0, 0, 0, 0);
+            if (S::row(i) < kStep && r < p.R && S::col(i) < p.D) {
+                qreg[i] = *reinterpret_cast<const uint4*>((const T*)p.q + row_at(p, p.vq, w.b, w.hk, r) + S::col(i));
+                dreg[i] = *reinterpret_cast<const uint4*>((const T*)p.dout + row_at(p, p.vd, w.b, w.hk, r) + S::col(i));
+            }
+        }
+        if (threadIdx.x < 2 * kStep) {                       // a row beyond the last: P = 2^(0 - inf) = 0, delta = 0
+            const int r = st * kStep + (int)(threadIdx.x & (kStep - 1));
+            lreg = threadIdx.x < kStep ? kInf : 0.f;
+            if (r < p.R) lreg = (threadIdx.x < kStep ? p.lse : p.delta)[bh * p.R + r];
+        }
+    };
+    if (st0 < st1) fetch(st0);
+    for (int st = st0; st < st1; ++st) {
+        const int buf = st & 1;
+        unsigned char *qt = Qs[buf], *dt = Ds[buf];
+        S::put(qt, qreg);
+        S::put(dt, dreg);
+        if (threadIdx.x < 2 * kStep) Ls[buf][threadIdx.x / kStep][threadIdx.x & (kStep - 1)] = lreg;
+        __syncthreads();
+        if (st + 1 < st1) fetch(st + 1);
+        if (!wave_on) continue;
+        // S and dP: rows on the registers, this lane's key
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+            const int at = l31 * S::kLd + (ks * 16 + h * 8) * 2;
+            s = E::mfma(*reinterpret_cast<const uint4*>(qt + at), kf[ks], s);
+            dp = E::mfma(*reinterpret_cast<const uint4*>(dt + at), vf[ks], dp);
+        }
+        float lse[16], del[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            *reinterpret_cast<float4*>(lse + 4 * g) = *reinterpret_cast<const float4*>(&Ls[buf][0][8 * g + 4 * h]);
+            *reinterpret_cast<float4*>(del + 4 * g) = *reinterpret_cast<const float4*>(&Ls[buf][1][8 * g + 4 * h]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float e = on ? __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse[i])) : 0.f;
+            s[i] = e;
+            dp[i] = e * (dp[i] - del[i]);
+        }
+        const int tr = (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint4 pf = pack_acc<E>(s, k), df = pack_acc<E>(dp, k);
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t) {
+                const int at = tr + (16 * k) * S::kLd + t * 64;
+                dv[t] = E::mfma(tr_pair(dt + at, dt + at + 8 * S::kLd), pf, dv[t]);
+                dk[t] = E::mfma(tr_pair(qt + at, qt + at + 8 * S::kLd), df, dk[t]);
+            }
+        }
+    }
+    if (key >= p.Lk) return;
+    const long at = (((long)w.b * p.Lk + key) * p.Hk + w.hk) * p.D;
+    const long whole = (long)p.B * p.Lk * p.Hk * p.D;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = t * 32 + 8 * g + 4 * h;
+            if (d >= p.D) continue;
+            if (p.splits > 1) {
+                float* o = p.part + (long)w.split * 2 * whole + at + d;
+                *reinterpret_cast<float4*>(o) = make_float4(dk[t][4 * g], dk[t][4 * g + 1], dk[t][4 * g + 2], dk[t][4 * g + 3]);
+                *reinterpret_cast<float4*>(o + whole) = make_float4(dv[t][4 * g], dv[t][4 * g + 1], dv[t][4 * g + 2], dv[t][4 * g + 3]);
+            } else {
+                uint2 u;
+                u.x = E::pair(dk[t][4 * g] * p.scale, dk[t][4 * g + 1] * p.scale);
+                u.y = E::pair(dk[t][4 * g + 2] * p.scale, dk[t][4 * g + 3] * p.scale);
+                *reinterpret_cast<uint2*>((T*)p.dk + at + d) = u;
+                u.x = E::pair(dv[t][4 * g], dv[t][4 * g + 1]);
+                u.y = E::pair(dv[t][4 * g + 2], dv[t][4 * g + 3]);
+                *reinterpret_cast<uint2*>((T*)p.dv + at + d) = u;
+            }
+        }
+}
+
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void xa_dq_kernel(Att p, int tiles) {
+    typedef typename E::raw T;
+    typedef Stage<DP, kKeys> S;
+    __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
+    __shared__ __attribute__((aligned(16))) unsigned char Vs[2][kKeys * S::kLd];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+    const Work w = work_of(p, tiles);
+    const int r = w.tile * kRows + wave * 32 + l31;
+    const bool row_on = r < p.R, wave_on = w.tile * kRows + wave * 32 < p.R;
+    const int len = key_count(p, w.b);
+    const int nkb = (len + kKeys - 1) / kKeys;
+    const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
+    const long bh = (long)w.b * p.Hk + w.hk;
+
+    uint4 qf[DP / 16], df[DP / 16];
+    row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r, row_on, qf);
+    row_operand<T, DP>(p, p.dout, p.vd, w.b, w.hk, r, row_on, df);
+    const float lse = row_on ? p.lse[bh * p.R + r] : kInf, del = row_on ? p.delta[bh * p.R + r] : 0.f;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
+
+    uint4 kreg[S::kPieces], vreg[S::kPieces];
+    unsigned long long set = 0, next = 0;
+    if (kb0 < kb1) {
+        next = key_set(p, w.b, len, kb0);
+        fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb0, next, kreg);
+        fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb0, next, vreg);
+    }
+    for (int kb = kb0; kb < kb1; ++kb) {
+        unsigned char *kt = Ks[kb & 1], *vt = Vs[kb & 1];
+        S::put(kt, kreg);
+        S::put(vt, vreg);
+        set = next;
+        __syncthreads();
+        if (kb + 1 < kb1) {
+            next = key_set(p, w.b, len, kb + 1);
+            fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb + 1, next, kreg);
+            fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb + 1, next, vreg);
+        }
+        if (!wave_on || set == 0) continue;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                const int at = (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
+                s = E::mfma(*reinterpret_cast<const uint4*>(kt + at), qf[ks], s);
+                dp = E::mfma(*reinterpret_cast<const uint4*>(vt + at), df[ks], dp);
+            }
+            const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float e = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse));
+                if (set != ~0ull) e = (bits >> entry(i, 0) & 1) ? e : 0.f;
+                s[i] = e * (dp[i] - del);
+            }
+            const unsigned char* kb_ = kt + (t * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd +
+                                       (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint4 sf = pack_acc<E>(s, k);
+#pragma unroll
+                for (int u = 0; u < DP / 32; ++u) {
+                    const unsigned char* a = kb_ + (16 * k) * S::kLd + u * 64;
+                    acc[u] = E::mfma(tr_pair(a, a + 8 * S::kLd), sf, acc[u]);
+                }
+            }
+        }
+    }
+    if (!row_on) return;
+    const long at = dense_row(p, w.b, w.hk, r);
+    const long whole = (long)p.B * p.Hk * p.R * p.D;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = t * 32 + 8 * g + 4 * h;
+            if (d >= p.D) continue;
+            if (p.splits > 1) {
+                *reinterpret_cast<float4*>(p.part + (long)w.split * whole + at + d) =
+                    make_float4(acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]);
+            } else {
+                uint2 u;
+                u.x = E::pair(acc[t][4 * g] * p.scale, acc[t][4 * g + 1] * p.scale);
+                u.y = E::pair(acc[t][4 * g + 2] * p.scale, acc[t][4 * g + 3] * p.scale);
+                *reinterpret_cast<uint2*>((T*)p.dq + at + d) = u;
+            }
+        }
+}
+
+// out[i] = factor * sum over parts of part[s][i], four elements a thread
+template <typename E>
+__global__ __launch_bounds__(256) void xa_sum_kernel(const float* part, long stride, int parts, long count, float factor,
+                                                     typename E::raw* out) {
+    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= count) return;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < parts; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(part + s * stride + i);
+        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+    uint2 u;
+    u.x = E::pair(a.x * factor, a.y * factor);
+    u.y = E::pair(a.z * factor, a.w * factor);
+    *reinterpret_cast<uint2*>(out + i) = u;
+}
+
+int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+
+// parts of a long axis of `steps` blocks: enough for about two workgroups a CU, at least four blocks a part
+int parts_for(long groups, long steps) {
+    long n = (512 + groups - 1) / groups;
+    const long most = (steps + 3) / 4;
+    if (n > most) n = most;
+    return (int)(n < 1 ? 1 : n);
+}
+
+struct Plan { long fwd_groups, dkv_groups; int rtiles, ktiles, fwd, dkv, dq, dp; };
+
+Plan plan_of(int B, long R, int Lk, int Hk, int D) {
+    Plan n;
+    n.dp = padded(D);
+    n.rtiles = (int)((R + kRows - 1) / kRows);
+    n.ktiles = (Lk + kRows - 1) / kRows;
+    n.fwd_groups = (long)B * Hk * n.rtiles;
+    n.dkv_groups = (long)B * Hk * n.ktiles;
+    n.fwd = n.dq = parts_for(n.fwd_groups, (Lk + kKeys - 1) / kKeys);
+    n.dkv = parts_for(n.dkv_groups, (R + kStep - 1) / kStep);
+    return n;
+}
+
+bool bad(int B, int Lq, int Lk, int Hk, int share, int D) {
+    return B <= 0 || Lq <= 0 || Lk <= 0 || Hk <= 0 || share <= 0 || D <= 0 || D % 8 || D > 128 ||
+           (long)Lq * share > 0x7fffff00L || (long)B * Hk * share > 0x7fffffffL || Lk > 0x7fffff00;
+}
+
+bool bad_grid(long n) { return n <= 0 || n > 0x7fffffffL; }
+
+template <typename E, int DP> int launch_fwd(Att p, const Plan& n, hipStream_t st) {
+    p.splits = n.fwd;
+    const long blocks = n.fwd_groups * n.fwd, rows = (long)p.B * p.Hk * p.R;
+    if (bad_grid(blocks) || bad_grid((rows + 3) / 4)) return -3;
+    xa_fwd_kernel<E, DP><<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.rtiles);
+    if (n.fwd > 1) xa_join_kernel<E, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, rows);
+    return DP_LAUNCH_STATUS();
+}
+
+template <typename E, int DP> int launch_bwd(Att p, const Plan& n, hipStream_t st) {
+    typedef typename E::raw T;
+    const long rows = (long)p.B * p.Hk * p.R, kv = (long)p.B * p.Lk * p.Hk * p.D, qn = rows * p.D;
+    if (bad_grid((rows + 15) / 16) || bad_grid(n.dkv_groups * n.dkv) || bad_grid(n.fwd_groups * n.dq) ||
+        bad_grid((kv + 1023) / 1024) || bad_grid((qn + 1023) / 1024))
+        return -3;
+    xa_delta_kernel<E><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, st>>>(p, rows);
+    p.splits = n.dkv;
+    xa_dkv_kernel<E, DP><<<dim3((unsigned)(n.dkv_groups * n.dkv)), 256, 0, st>>>(p, n.ktiles);
+    if (n.dkv > 1) {
+        const dim3 g((unsigned)((kv + 1023) / 1024));
+        xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part, 2 * kv, n.dkv, kv, p.scale, (T*)p.dk);
+        xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part + kv, 2 * kv, n.dkv, kv, 1.f, (T*)p.dv);
+    }
+    p.splits = n.dq;
+    xa_dq_kernel<E, DP><<<dim3((unsigned)(n.fwd_groups * n.dq)), 256, 0, st>>>(p, n.rtiles);
+    if (n.dq > 1)
+        xa_sum_kernel<E><<<dim3((unsigned)((qn + 1023) / 1024)), 256, 0, st>>>(p.part, qn, n.dq, qn, p.scale, (T*)p.dq);
+    return DP_LAUNCH_STATUS();
+}
+
+template <template <typename, int> class Run> int dispatch(int fp16, int dp, const Att& p, const Plan& n, hipStream_t st) {
+    switch (dp + fp16) {
+        case 32: return Run<Bf, 32>::go(p, n, st);
+        case 33: return Run<Hf, 32>::go(p, n, st);
+        case 64: return Run<Bf, 64>::go(p, n, st);
+        case 65: return Run<Hf, 64>::go(p, n, st);
+        case 96: return Run<Bf, 96>::go(p, n, st);
+        case 97: return Run<Hf, 96>::go(p, n, st);
+        case 128: return Run<Bf, 128>::go(p, n, st);
+        case 129: return Run<Hf, 128>::go(p, n, st);
+    }
+    return -1;
+}
+
+template <typename E, int DP> struct RunFwd {
+    static int go(const Att& p, const Plan& n, hipStream_t st) { return launch_fwd<E, DP>(p, n, st); }
+};
+template <typename E, int DP> struct RunBwd {
+    static int go(const Att& p, const Plan& n, hipStream_t st) { return launch_bwd<E, DP>(p, n, st); }
+};
+
+bool misaligned(const void* p, const long* s) { return ((uintptr_t)p & 15) || s[0] % 8 || s[1] % 8 || s[2] % 8; }
+
+}  // namespace
+
+// floats of workspace for the parts of split axes (0: none); backward's covers dk and dv, then dq
+DP_EXPORT long dp_xa_workspace(int B, int Lq, int Lk, int Hk, int share, int D, int backward) {
+    if (bad(B, Lq, Lk, Hk, share, D)) return -1;
+    const long R = (long)Lq * share;
+    const Plan n = plan_of(B, R, Lk, Hk, D);
+    if (!backward) return n.fwd > 1 ? (long)B * Hk * n.fwd * R * (n.dp + 2) : 0;
+    const long a = n.dkv > 1 ? 2L * n.dkv * B * Lk * Hk * D : 0, b = n.dq > 1 ? (long)n.dq * B * Hk * R * D : 0;
+    return a > b ? a : b;
+}
+
+// strides: image, position and head of q, k and v (nine), in elements
+DP_EXPORT int dp_xa_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int* lens,
+                        const void* mask, long mask_ld, float* ws, const long* strides, int B, int Lq, int Lk, int Hk,
+                        int share, int D, float scale, int fp16, void* stream) {
+    if (bad(B, Lq, Lk, Hk, share, D) || !q || !k || !v || !out || !strides || misaligned(q, strides) ||
+        misaligned(k, strides + 3) || misaligned(v, strides + 6) || ((uintptr_t)out & 15) || !(scale > 0.f))
+        return -2;
+    Att p{};
+    p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse; p.lens = lens; p.mask = (const unsigned char*)mask; p.mask_ld = mask_ld;
+    p.vq = {strides[0], strides[1], strides[2]}; p.vk = {strides[3], strides[4], strides[5]};
+    p.vv = {strides[6], strides[7], strides[8]};
+    p.B = B; p.Lq = Lq; p.Lk = Lk; p.Hk = Hk; p.share = share; p.D = D; p.R = Lq * share;
+    p.scale = scale; p.c = scale * 1.4426950408889634f; p.part = ws;
+    const Plan n = plan_of(B, p.R, Lk, Hk, D);
+    if (n.fwd > 1 && !ws) return -2;
+    return dispatch<RunFwd>(fp16, n.dp, p, n, (hipStream_t)stream);
+}
+
+// strides: image, position and head of q, k, v and dout (twelve); o and the gradients are dense; delta: scratch like lse
+DP_EXPORT int dp_xa_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+                        float* delta, void* dq, void* dk, void* dv, const int* lens, const void* mask, long mask_ld,
+                        float* ws, const long* strides, int B, int Lq, int Lk, int Hk, int share, int D, float scale,
+                        int fp16, void* stream) {
+    if (bad(B, Lq, Lk, Hk, share, D) || !q || !k || !v || !o || !dout || !lse || !delta || !dq || !dk || !dv || !strides ||
+        misaligned(q, strides) || misaligned(k, strides + 3) || misaligned(v, strides + 6) || misaligned(dout, strides + 9) ||
+        (((uintptr_t)o | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) || !(scale > 0.f))
+        return -2;
+    Att p{};
+    p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta;
+    p.dq = dq; p.dk = dk; p.dv = dv; p.lens = lens; p.mask = (const unsigned char*)mask; p.mask_ld = mask_ld;
+    p.vq = {strides[0], strides[1], strides[2]}; p.vk = {strides[3], strides[4], strides[5]};
+    p.vv = {strides[6], strides[7], strides[8]}; p.vd = {strides[9], strides[10], strides[11]};
+    p.B = B; p.Lq = Lq; p.Lk = Lk; p.Hk = Hk; p.share = share; p.D = D; p.R = Lq * share;
+    p.scale = scale; p.c = scale * 1.4426950408889634f; p.part = ws;
+    const Plan n = plan_of(B, p.R, Lk, Hk, D);
+    if ((n.dkv > 1 || n.dq > 1) && !ws) return -2;
+    return dispatch<RunBwd>(fp16, n.dp, p, n, (hipStream_t)stream);
+}

@@ -10,6 +10,7 @@ from .batchnorm import (BatchNorm2d, batch_norm_act, convert_sync_batchnorm,  # 
                         freeze_batchnorm)
 from .bnfold import conv_bn_add_relu  # noqa: F401
 from .conv import Conv2d, conv2d, conv_bn_act, conv_out_size  # noqa: F401
+from .cross_attention import cross_attention  # noqa: F401
 from .dropout import dropout  # noqa: F401
 from .group_norm import group_norm_act  # noqa: F401
 from .loss import SoftmaxCrossEntropy, softmax_cross_entropy  # noqa: F401

@@ -1,0 +1,242 @@
+"""Cross attention kernels (csrc/cross_attention.hip) against a 64-bit definition.
+
+Tolerances.  u = 2^-24, h = half a step of the type (bf16 2^-8, fp16 2^-11), n = terms of a sum.  A product summed in 32
+bits is off by at most n u times the sum of the terms' magnitudes.  A score off by e changes a probability by a factor
+1 + 2 e (numerator and denominator); exponents carry a few u of their size.  P and dS are rounded once (h, and in fp16 at
+most 2^-25 absolute below its smallest normal value), delta is taken from the rounded output, outputs are rounded once.
+"""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def _inputs(b, lq, lk, hq, hk, d, dtype, seed, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    mk = lambda n, h, s=1.0: (torch.randn(b, n, h, d, generator=g, device="cuda") * s).to(dtype)  # noqa: E731
+    return mk(lq, hq, spread), mk(lk, hk, spread), mk(lk, hk), mk(lq, hq)
+
+
+def _check(q, k, v, dout, lens=None, mask=None, scale=None, train=True):
+    from distributedpytorch_amd import ops
+    b, lq, hq, d = q.shape
+    lk, hk = k.shape[1], k.shape[2]
+    dtype = q.dtype
+    half = torch.finfo(dtype).eps / 2
+    sub = torch.finfo(dtype).smallest_normal * half
+    on = torch.ones(b, lk, dtype=torch.bool, device="cuda")
+    if lens is not None:
+        on &= torch.arange(lk, device="cuda") < lens[:, None]
+    if mask is not None:
+        on &= mask
+    leaves = [t.detach().requires_grad_(train) for t in (q, k, v)]
+    out = ops.cross_attention(*leaves, key_lengths=lens, key_mask=mask, scale=scale)
+    assert out.shape == q.shape and out.dtype == dtype
+    grads = torch.autograd.grad(out, leaves, dout) if train else ()
+    sc = 1 / math.sqrt(d) if scale is None else scale
+    want = [torch.zeros(t.shape, dtype=torch.float64, device="cuda") for t in (q, q, k, v)]
+    tol = [torch.full_like(t, 2 * sub) for t in want]
+    for i in range(b):
+        idx = on[i].nonzero().flatten()
+        if idx.numel() == 0:
+            continue
+        for j in range(hq):
+            m = j // (hq // hk)
+            qq, do = q[i, :, j].double(), dout[i, :, j].double()
+            kk, vv = k[i, idx, m].double(), v[i, idx, m].double()
+            n = idx.numel()
+            s = qq @ kk.t() * sc
+            p = torch.softmax(s, dim=1)
+            o = p @ vv
+            es = (d + 3) * U * (qq.abs() @ kk.abs().t()) * sc + 8 * U * (1 + s.abs())
+            es = 2 * es.max(dim=1, keepdim=True)[0] * 1.1
+            ep = p * (half + es) + sub                              # of a rounded probability
+            eo = ep @ vv.abs() + (n + 8) * U * (p @ vv.abs()) + half * o.abs() + sub
+            want[0][i, :, j], tol[0][i, :, j] = o, tol[0][i, :, j] + eo
+            dp = do @ vv.t()
+            delta = (do * o).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            edp = (d + 1) * U * (do.abs() @ vv.abs().t())
+            edelta = (do.abs() * eo).sum(1, keepdim=True) + (d + 1) * U * (do.abs() * o.abs()).sum(1, keepdim=True)
+            eds = p * (edp + edelta) * (1 + es) + ds.abs() * (es + half + 4 * U) + sub
+            want[1][i, :, j] = ds @ kk * sc
+            tol[1][i, :, j] += sc * (eds @ kk.abs() + (n + 8) * U * (ds.abs() @ kk.abs()))
+            want[2][i, idx, m] += ds.t() @ qq * sc
+            want[3][i, idx, m] += p.t() @ do
+            r = lq * (hq // hk) + 8
+            tol[2][i, idx, m] += sc * (eds.t() @ qq.abs() + r * U * (ds.abs().t() @ qq.abs()))
+            tol[3][i, idx, m] += ep.t() @ do.abs() + r * U * (p.t() @ do.abs())
+    for name, got, w, t in zip(("out", "dq", "dk", "dv"), (out, *grads), want, tol):
+        err = (got.double() - w).abs()
+        t = t + half * w.abs() if name != "out" else t
+        bad = ~(err <= t)
+        assert not bad.any(), (name, int(bad.sum()), float((err / t).max()))
+    if train:
+        off = ~on
+        assert (grads[1][off] == 0).all() and (grads[2][off] == 0).all()
+    return out
+
+
+SHAPES = [  # b, lq, lk, hq, hk, d
+    (1, 1, 1, 1, 1, 8), (2, 1, 64, 4, 4, 64), (1, 1, 65, 8, 2, 128), (2, 31, 33, 2, 2, 32), (1, 128, 64, 2, 1, 64),
+    (2, 129, 63, 4, 2, 64), (1, 127, 257, 3, 3, 40), (2, 200, 130, 6, 2, 96), (1, 300, 1, 4, 1, 128), (3, 5, 1000, 2, 2, 80),
+    (1, 1000, 31, 8, 8, 128), (1, 77, 129, 12, 3, 16),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_cross_attention_shapes(shape, dtype):
+    _check(*_inputs(*shape, dtype, seed=sum(shape)))
+
+
+@pytest.mark.parametrize("shape", [(4, 70, 150, 4, 2, 64), (4, 1, 300, 8, 2, 128), (4, 33, 129, 2, 2, 96)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["lengths", "mask", "both"])
+def test_cross_attention_lengths_and_masks(shape, dtype, kind):
+    q, k, v, dout = _inputs(*shape, dtype, seed=7)
+    lk = shape[2]
+    lens = mask = None
+    if kind != "mask":
+        lens = torch.tensor([lk, 0, 1, lk - 7], dtype=torch.int32, device="cuda")
+    if kind != "lengths":
+        g = torch.Generator().manual_seed(1)
+        mask = (torch.rand(4, lk, generator=g) < 0.5).cuda()
+        mask[3] = False
+        mask[0, 64:128] = False                                     # a whole block of keys
+    out = _check(q, k, v, dout, lens, mask)
+    if kind != "lengths":
+        assert (out[3] == 0).all()
+    if lens is not None:
+        assert (out[1] == 0).all()
+        # the values behind a sequence, and lengths outside [0, Lk], change nothing
+        wide = torch.tensor([lk + 5, -3, 1, lk - 7], device="cuda")
+        k2, v2 = k.clone(), v.clone()
+        k2[3, lk - 7:], v2[3, lk - 7:] = float("nan"), float("inf")
+        k2[1], v2[1] = float("inf"), float("nan")
+        from distributedpytorch_amd import ops
+        a = ops.cross_attention(q, k2, v2, key_lengths=wide, key_mask=mask)
+        assert torch.equal(a, out)
+        assert torch.equal(ops.cross_attention(q, k2, v2, key_lengths=wide.int(), key_mask=mask), out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_cross_attention_junk_in_masked_places_leaves_gradients_alone(dtype):
+    from distributedpytorch_amd import ops
+    q, k, v, dout = _inputs(2, 40, 200, 4, 2, 64, dtype, seed=11)
+    g = torch.Generator().manual_seed(2)
+    mask = (torch.rand(2, 200, generator=g) < 0.5).cuda()
+    grads = []
+    for junk in (0.0, float("nan"), float("-inf"), torch.finfo(dtype).min, torch.finfo(dtype).max):
+        ks, vs = (torch.where(mask[:, :, None, None], t, torch.full_like(t, junk)).requires_grad_(True) for t in (k, v))
+        qs = q.detach().requires_grad_(True)
+        out = ops.cross_attention(qs, ks, vs, key_mask=mask)
+        grads.append((out.detach(),) + torch.autograd.grad(out, (qs, ks, vs), dout))
+    for other in grads[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(grads[0], other))
+    assert all(torch.isfinite(t).all() for t in grads[0])
+
+
+@pytest.mark.parametrize("spread,scale", [(6.0, None), (1.0, 3.0), (0.01, None)])
+def test_cross_attention_peaked_and_flat_rows(spread, scale):
+    _check(*_inputs(1, 100, 500, 2, 2, 64, torch.bfloat16, 5, spread), scale=scale)
+
+
+def test_cross_attention_rising_scores_move_the_maximum_every_block():
+    q, k, v, dout = _inputs(1, 64, 640, 1, 1, 64, torch.bfloat16, 6)
+    ramp = torch.linspace(0.0, 4.0, 640, device="cuda").to(torch.bfloat16)
+    q = torch.ones_like(q)
+    k = (ramp[None, :, None, None].expand(k.shape) * 1.0).contiguous()
+    _check(q, k, v, dout)
+
+
+def test_cross_attention_views():
+    from distributedpytorch_amd import ops
+    n, c, heads = 2, 128, 4
+    fine = torch.randn(n, c, 9, 7, device="cuda").to(torch.bfloat16).contiguous(memory_format=torch.channels_last)
+    coarse = torch.randn(n, 2 * c, 5, 3, device="cuda").to(torch.bfloat16).contiguous(memory_format=torch.channels_last)
+    seq = lambda t: t.permute(0, 2, 3, 1).reshape(n, -1, heads, t.shape[1] // heads)  # noqa: E731
+    q = seq(fine)
+    k, v = seq(coarse[:, :c]), seq(coarse[:, c:])                    # one projection holds both: rows of 2 C elements
+    assert q.data_ptr() == fine.data_ptr() and k.stride(1) == 2 * c
+    dout = torch.randn(n, 63, heads, 32, device="cuda").to(torch.bfloat16)
+    _check(q, k, v, dout)
+    _check(q, k, v, dout.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3))        # heads first in memory
+    _check(q, k, v, torch.ones(1, 1, 1, 1, device="cuda", dtype=torch.bfloat16).expand(n, 63, heads, 32))
+    _check(q[..., 1:], k[..., 1:], v[..., 1:], dout[..., 1:])        # rows off 16 bytes and a width of 31
+    _check(q, k[:1].expand(n, -1, -1, -1), v[:1].expand(n, -1, -1, -1), dout)         # one image's keys for all
+    with pytest.raises(NotImplementedError):
+        ops.cross_attention(*(torch.zeros(1, 2, 1, 136, device="cuda", dtype=torch.bfloat16),) * 3)
+    with pytest.raises(TypeError):
+        ops.cross_attention(*(torch.zeros(1, 2, 1, 64, device="cuda"),) * 3)
+
+
+def test_cross_attention_broadcast_keys_sum_their_gradient():
+    from distributedpytorch_amd import ops
+    q, k, v, dout = _inputs(3, 50, 70, 2, 2, 64, torch.bfloat16, 8)
+    k1, v1 = k[:1].detach().requires_grad_(True), v[:1].detach().requires_grad_(True)
+    out = ops.cross_attention(q, k1.expand(3, -1, -1, -1), v1.expand(3, -1, -1, -1))
+    gk, gv = torch.autograd.grad(out, (k1, v1), dout)
+    kf, vf = k[:1].expand(3, -1, -1, -1).contiguous().requires_grad_(True), v[:1].expand(3, -1, -1, -1).contiguous().requires_grad_(True)
+    hk, hv = torch.autograd.grad(ops.cross_attention(q, kf, vf), (kf, vf), dout)
+    assert torch.equal(gk, hk.sum(0, keepdim=True)) and torch.equal(gv, hv.sum(0, keepdim=True))
+
+
+def test_cross_attention_long_axes_split_and_repeat():
+    """Few rows over many keys, and many rows over few keys: both axes run in parts, joined in one order."""
+    from distributedpytorch_amd import ops
+    for shape in ((1, 3, 9001, 2, 1, 64), (1, 9001, 3, 2, 1, 64)):
+        q, k, v, dout = _inputs(*shape, torch.bfloat16, 9)
+        _check(q, k, v, dout)
+        runs = []
+        for _ in range(2):
+            ls = [t.detach().requires_grad_(True) for t in (q, k, v)]
+            out = ops.cross_attention(*ls)
+            runs.append((out.detach(),) + torch.autograd.grad(out, ls, dout))
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("shape", [(2, 65, 130, 4, 2, 64), (2, 1, 3000, 4, 2, 64)])
+def test_cross_attention_replays(shape):
+    from distributedpytorch_amd import ops
+    q, k, v, dout = _inputs(*shape, torch.bfloat16, 10)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    lens = torch.tensor([shape[2], shape[2] // 2], dtype=torch.int32, device="cuda")
+
+    def step():
+        out = ops.cross_attention(*leaves, key_lengths=lens)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        with torch.no_grad():
+            for t, n in zip(leaves, _inputs(*shape, torch.bfloat16, 20 + i)):
+                t.copy_(n)
+            lens.copy_(torch.tensor([shape[2] - i, i], dtype=torch.int32))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_cross_attention_without_a_graph_equals_with_one():
+    from distributedpytorch_amd import ops
+    q, k, v, _ = _inputs(2, 70, 90, 2, 2, 64, torch.float16, 12)
+    with torch.no_grad():
+        a = ops.cross_attention(q, k, v)
+    assert torch.equal(a, ops.cross_attention(q.requires_grad_(True), k, v))
