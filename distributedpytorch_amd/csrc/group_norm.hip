@@ -77,22 +77,22 @@ __device__ __forceinline__ Place place(const Geo& g) {
     return p;
 }
 
-// sum of acc[0..K) over the rpp threads that share a pack; the result is left with the threads of lane_row 0
-template <int K> __device__ __forceinline__ void join_rows(float* acc, float* lds, const Geo& g, const Place& p) {
+// sum of acc[0..K) over the `rows` lines of `cols` threads of a block of N; the result is left with the first line
+template <int K, int N> __device__ __forceinline__ void join_rows(float* acc, float* lds, int cols, int rows, int line) {
     const int tid = threadIdx.x;
 #pragma unroll
-    for (int k = 0; k < K; ++k) lds[k * 256 + tid] = acc[k];
+    for (int k = 0; k < K; ++k) lds[k * N + tid] = acc[k];
     int s = 1;
-    while (s < g.rpp) s <<= 1;
+    while (s < rows) s <<= 1;
     for (s >>= 1; s > 0; s >>= 1) {
         __syncthreads();
-        if (p.lane_row < s && p.lane_row + s < g.rpp)
+        if (line < s && line + s < rows)
 #pragma unroll
-            for (int k = 0; k < K; ++k) lds[k * 256 + tid] += lds[k * 256 + tid + s * g.cb];
+            for (int k = 0; k < K; ++k) lds[k * N + tid] += lds[k * N + tid + s * cols];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) acc[k] = lds[k * 256 + tid];
+    for (int k = 0; k < K; ++k) acc[k] = lds[k * N + tid];
 }
 
 constexpr int kUnroll = 4;   // packs in flight per thread and operand
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(Geo g, const T* __restric
                     }
         }
     }
-    join_rows<2 * V>(acc, lds, g, p);
+    join_rows<2 * V, 256>(acc, lds, g.cb, g.rpp, p.lane_row);
     if (p.on && p.lane_row == 0) {
         float* o = part + ((p.n * g.splits + p.split) * 2) * g.C + (long)p.chunk * V;
 #pragma unroll
@@ -149,42 +149,75 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     return v;
 }
 
-// one wave per (image, group): stats[n, g] = (mean, rstd)
-__global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long waves, const float* __restrict__ part,
+// A team of `wide` waves (1 or 4, whole in one block of 256 threads) takes one (image, group): its items are the group's
+// (row range, channel) pairs, in memory order.
+struct Team { long gi, n; int c0, items, first, step; bool on; };
+
+__device__ __forceinline__ Team team_of(const Geo& g, long groups, int wide, long block) {
+    const int tid = threadIdx.x;
+    Team t;
+    t.step = wide * 64;
+    t.gi = block * (4 / wide) + tid / t.step;
+    t.on = t.gi < groups;
+    t.n = t.on ? t.gi / g.G : 0;
+    t.c0 = t.on ? (int)(t.gi % g.G) * g.cpg : 0;
+    t.items = t.on ? g.cpg * g.splits : 0;
+    t.first = tid % t.step;
+    return t;
+}
+
+__device__ __forceinline__ double team_sum(double v, int wide, double* lds) {
+    v = wave_sum_d(v);
+    if (wide == 1) return v;
+    const int w = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[w] = v;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// stats[n, g] = (mean, rstd).  Every item is a sample with a mean and squared deviations of its own; all the terms that
+// join them are positive.
+__global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int wide, const float* __restrict__ part,
                                                         const float* __restrict__ pivot, double* __restrict__ stats) {
-    const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (w >= waves) return;
-    const long n = w / g.G;
-    const int c0 = (int)(w % g.G) * g.cpg;
-    const double inv = 1.0 / (double)g.hw;
+    __shared__ double lds[4];
+    const Team t = team_of(g, groups, wide, blockIdx.x);
+    const float* base = part + t.n * g.splits * 2 * g.C + t.c0;
+    const float* pv = pivot + t.n * g.C + t.c0;
     double sm = 0.0;
-    for (int c = lane; c < g.cpg; c += 64) {
-        const float* q = part + n * g.splits * 2 * g.C + c0 + c;
-        double s1 = 0.0;
-        for (int s = 0; s < g.splits; ++s) s1 += (double)q[(long)s * 2 * g.C];
-        sm += (double)pivot[n * g.C + c0 + c] + s1 * inv;
+#pragma unroll 4
+    for (int i = t.first; i < t.items; i += t.step) {
+        const int s = i / g.cpg, c = i - s * g.cpg;
+        const long rows = (s + 1) * g.rows < g.hw ? g.rows : g.hw - s * g.rows;
+        sm += (double)rows * (double)pv[c] + (double)base[(long)s * 2 * g.C + c];
     }
-    const double mean = wave_sum_d(sm) / g.cpg;
+    const double count = (double)g.hw * g.cpg;
+    const double mean = team_sum(sm, wide, lds) / count;
     double m2 = 0.0;
-    for (int c = lane; c < g.cpg; c += 64) {
-        const float* q = part + n * g.splits * 2 * g.C + c0 + c;
-        double s1 = 0.0, s2 = 0.0;
-        for (int s = 0; s < g.splits; ++s) { s1 += (double)q[(long)s * 2 * g.C]; s2 += (double)q[(long)s * 2 * g.C + g.C]; }
-        const double d = (double)pivot[n * g.C + c0 + c] + s1 * inv - mean;
-        const double own = s2 - s1 * s1 * inv;
-        m2 += (own > 0.0 ? own : (own != own ? own : 0.0)) + d * d * (double)g.hw;      // (a NaN stays one)
+#pragma unroll 4
+    for (int i = t.first; i < t.items; i += t.step) {
+        const int s = i / g.cpg, c = i - s * g.cpg;
+        const double rows = (double)((s + 1) * g.rows < g.hw ? g.rows : g.hw - s * g.rows);
+        const double s1 = (double)base[(long)s * 2 * g.C + c], s2 = (double)base[(long)s * 2 * g.C + g.C + c];
+        const double own = s2 - s1 * s1 / rows, d = (double)pv[c] + s1 / rows - mean;
+        m2 += (own < 0.0 ? 0.0 : own) + d * d * rows;                                   // (a NaN stays one)
     }
-    m2 = wave_sum_d(m2);
-    if (lane == 0) {
-        const double var = m2 / ((double)g.hw * g.cpg);
-        stats[2 * w] = mean;
-        stats[2 * w + 1] = 1.0 / sqrt(var + (double)g.eps);
+    m2 = team_sum(m2, wide, lds);
+    if (t.on && t.first == 0) {
+        stats[2 * t.gi] = mean;
+        stats[2 * t.gi + 1] = 1.0 / sqrt(m2 / count + (double)g.eps);
     }
 }
 
 // per-channel constants of one thread
 template <int V> struct Coef { float ah[V], al[V], bh[V], bl[V]; };        // z = x a + b (+ residual)
+
+template <int V>
+__device__ __forceinline__ void coef_of(Coef<V>& c, int i, double mean, double rstd, double w, double b) {
+    const double a = w * rstd, bb = b - mean * a;
+    c.ah[i] = (float)a; c.al[i] = (float)(a - (double)c.ah[i]);
+    c.bh[i] = (float)bb; c.bl[i] = (float)(bb - (double)c.bh[i]);
+}
 
 template <int V>
 __device__ __forceinline__ Coef<V> coef(const Geo& g, const Place& p, const double* stats, const float* w, const float* b) {
@@ -193,9 +226,7 @@ __device__ __forceinline__ Coef<V> coef(const Geo& g, const Place& p, const doub
     for (int i = 0; i < V; ++i) {
         const int ch = p.chunk * V + i;
         const double* st = stats + 2 * (p.n * g.G + ch / g.cpg);
-        const double a = (w ? (double)w[ch] : 1.0) * st[1], bb = (b ? (double)b[ch] : 0.0) - st[0] * a;
-        c.ah[i] = (float)a; c.al[i] = (float)(a - (double)c.ah[i]);
-        c.bh[i] = (float)bb; c.bl[i] = (float)(bb - (double)c.bh[i]);
+        coef_of(c, i, st[0], st[1], w ? (double)w[ch] : 1.0, b ? (double)b[ch] : 0.0);
     }
     return c;
 }
@@ -317,7 +348,7 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __re
                     }
         }
     }
-    join_rows<2 * V>(acc, lds, g, p);
+    join_rows<2 * V, 256>(acc, lds, g.cb, g.rpp, p.lane_row);
     if (p.on && p.lane_row == 0) {
         float* o = part + ((p.n * g.splits + p.split) * 2) * g.C + (long)p.chunk * V;
 #pragma unroll
@@ -325,38 +356,48 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __re
     }
 }
 
-// blocks [0, gblocks): one wave per (image, group) -> means[n, g] = (m1, m2); the rest: one thread per channel -> dw, db
-__global__ __launch_bounds__(256) void gn_bwd_finish_kernel(Geo g, long images, int gblocks, const float* __restrict__ part,
-                                                            const float* __restrict__ w, float* __restrict__ means,
-                                                            float* __restrict__ dw, float* __restrict__ db) {
-    if ((int)blockIdx.x < gblocks) {
-        const long wv = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-        const int lane = threadIdx.x & 63;
-        if (wv >= images * g.G) return;
-        const long n = wv / g.G;
-        const int c0 = (int)(wv % g.G) * g.cpg;
-        double a = 0.0, q = 0.0;
-        for (int c = lane; c < g.cpg; c += 64) {
-            const float* s = part + n * g.splits * 2 * g.C + c0 + c;
-            double s1 = 0.0, s2 = 0.0;
-            for (int k = 0; k < g.splits; ++k) { s1 += (double)s[(long)k * 2 * g.C]; s2 += (double)s[(long)k * 2 * g.C + g.C]; }
-            const double wc = w ? (double)w[c0 + c] : 1.0;
-            a += wc * s1; q += wc * s2;
-        }
-        a = wave_sum_d(a); q = wave_sum_d(q);
-        if (lane == 0) {
-            const double inv = 1.0 / ((double)g.hw * g.cpg);
-            means[2 * wv] = (float)(a * inv);
-            means[2 * wv + 1] = (float)(q * inv);
-        }
-        return;
+// means[n, g] = (m1, m2)
+__global__ __launch_bounds__(256) void gn_bwd_means_kernel(Geo g, long groups, int wide, const float* __restrict__ part,
+                                                           const float* __restrict__ w, float* __restrict__ means) {
+    __shared__ double lds[4];
+    const Team t = team_of(g, groups, wide, blockIdx.x);
+    const float* base = part + t.n * g.splits * 2 * g.C + t.c0;
+    double a = 0.0, q = 0.0;
+#pragma unroll 4
+    for (int i = t.first; i < t.items; i += t.step) {
+        const int s = i / g.cpg, c = i - s * g.cpg;
+        const double wc = w ? (double)w[t.c0 + c] : 1.0;
+        a += wc * (double)base[(long)s * 2 * g.C + c];
+        q += wc * (double)base[(long)s * 2 * g.C + g.C + c];
     }
-    const int c = ((int)blockIdx.x - gblocks) * 256 + threadIdx.x;
-    if (c >= g.C) return;
+    a = team_sum(a, wide, lds);
+    q = team_sum(q, wide, lds);
+    if (t.on && t.first == 0) {
+        const double inv = 1.0 / ((double)g.hw * g.cpg);
+        means[2 * t.gi] = (float)(a * inv);
+        means[2 * t.gi + 1] = (float)(q * inv);
+    }
+}
+
+// dw and db: 16 channels by 64 lines of parts a block
+__global__ __launch_bounds__(1024) void gn_bwd_params_kernel(int C, long lines, const float* __restrict__ part,
+                                                             float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ double lds[2][1024];
+    const int tid = threadIdx.x, c = blockIdx.x * 16 + (tid & 15);
     double s1 = 0.0, s2 = 0.0;
-    for (long k = 0; k < images * g.splits; ++k) { s1 += (double)part[2 * k * g.C + c]; s2 += (double)part[(2 * k + 1) * g.C + c]; }
-    if (dw) dw[c] = (float)s2;
-    if (db) db[c] = (float)s1;
+    if (c < C)
+#pragma unroll 8
+        for (long k = tid >> 4; k < lines; k += 64) { s1 += (double)part[2 * k * C + c]; s2 += (double)part[(2 * k + 1) * C + c]; }
+    lds[0][tid] = s1;
+    lds[1][tid] = s2;
+    for (int s = 512; s >= 16; s >>= 1) {
+        __syncthreads();
+        if (tid < s) { lds[0][tid] += lds[0][tid + s]; lds[1][tid] += lds[1][tid + s]; }
+    }
+    if (tid < 16 && c < C) {
+        if (dw) dw[c] = (float)lds[1][tid];
+        if (db) db[c] = (float)lds[0][tid];
+    }
 }
 
 template <typename T, int V, int ACT, bool RES>
@@ -415,6 +456,194 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
     }
 }
 
+// ------------------------------------------------------------------------------------------------ groups that fit a block
+// Where a group's map fits the registers of one block (at most kHeld packs for each of its 512 threads), the block reads
+// it once, takes the statistics from its registers (the mean first, then the squared differences from it) and writes the
+// result: one launch forward, and no second read.  Needs whole packs inside a group (cpg a multiple of V).
+constexpr int kBlock = 512, kHeld = 16;
+
+struct Slab { long n; int chunk, row, rows; bool on; };
+
+__device__ __forceinline__ Slab slab_of(const Geo& g, long id) {
+    const int cw = g.cv;                                  // packs of a group's row (make_slab)
+    Slab s;
+    s.n = id / g.G;
+    s.rows = kBlock / cw;
+    s.row = (int)threadIdx.x / cw;
+    s.chunk = (int)(id % g.G) * cw + (int)threadIdx.x % cw;
+    s.on = s.row < s.rows;
+    return s;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+    v = wave_sum_d(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double t = 0.0;
+#pragma unroll
+    for (int i = 0; i < kBlock / 64; ++i) t += lds[i];
+    return t;
+}
+
+template <typename T, int V, int K>
+__device__ __forceinline__ void slab_load(Pack<T, V> (&a)[K], const T* base, long ld, const Geo& g, const Slab& s) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long r = s.row + (long)k * s.rows;
+        if (s.on && r < g.hw) a[k] = load_pack<T, V>(base + (s.n * g.hw + r) * ld + (long)s.chunk * V);
+    }
+}
+
+template <typename T, int V, int ACT, bool RES, int K>
+__global__ __launch_bounds__(kBlock) void gn_slab_fwd_kernel(Geo g, const T* __restrict__ x, const T* __restrict__ res,
+                                                             const float* __restrict__ w, const float* __restrict__ b,
+                                                             T* __restrict__ y, double* __restrict__ stats) {
+    constexpr bool kExact = sizeof(T) == 4;
+    __shared__ double lds[kBlock / 64];
+    const long id = blockIdx.x;
+    const Slab s = slab_of(g, id);
+    Pack<T, V> a[K], e[K];
+    slab_load<T, V, K>(a, x, g.ldx, g, s);
+    if constexpr (RES) slab_load<T, V, K>(e, res, g.ldr, g, s);
+    const double inv = 1.0 / ((double)g.hw * g.cpg);
+    // differences from the thread's own first element, so that a mean far above the spread costs no bits
+    const float first = s.on && s.row < g.hw ? to_f(a[0].v[0]) : 0.f;
+    float sum = 0.f;
+    int held = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (s.on && s.row + (long)k * s.rows < g.hw) {
+            held += V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum += to_f(a[k].v[i]) - first;
+        }
+    const double mean = block_sum((double)sum + (double)held * (double)first, lds) * inv;
+    const float mh = (float)mean, ml = (float)(mean - (double)mh);
+    float sq = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (s.on && s.row + (long)k * s.rows < g.hw)
+#pragma unroll
+            for (int i = 0; i < V; ++i) { const float d = (to_f(a[k].v[i]) - mh) - ml; sq = fmaf(d, d, sq); }
+    const double rstd = 1.0 / sqrt(block_sum((double)sq, lds) * inv + (double)g.eps);
+    if (threadIdx.x == 0) { stats[2 * id] = mean; stats[2 * id + 1] = rstd; }
+    if (!s.on) return;
+    Coef<V> cf;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int ch = s.chunk * V + i;
+        coef_of(cf, i, mean, rstd, w ? (double)w[ch] : 1.0, b ? (double)b[ch] : 0.0);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long r = s.row + (long)k * s.rows;
+        if (r < g.hw) {
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float z = affine(to_f(a[k].v[i]), cf.ah[i], cf.al[i], cf.bh[i], cf.bl[i]);
+                if constexpr (RES) z += to_f(e[k].v[i]);
+                f[i] = act_fwd<ACT, kExact>(z);
+            }
+            store_pack<T, V>(y + (s.n * g.hw + r) * g.C + (long)s.chunk * V, f);
+        }
+    }
+}
+
+// part[n, 0 | 1, c] = sum dz | sum dz xhat of the image, for dw and db
+template <typename T, int V, int ACT, bool RES, int K>
+__global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __restrict__ dy, const T* __restrict__ x,
+                                                             const T* __restrict__ res, const float* __restrict__ w,
+                                                             const float* __restrict__ b,
+                                                             const double* __restrict__ stats, T* __restrict__ dx,
+                                                             T* __restrict__ dres, float* __restrict__ part) {
+    constexpr bool kExact = sizeof(T) == 4, kAct = ACT != kNone;
+    __shared__ float lds[2 * V * kBlock];
+    __shared__ double sums[kBlock / 64];
+    const long id = blockIdx.x;
+    const Slab s = slab_of(g, id);
+    Pack<T, V> a[K], d[K], e[K];
+    slab_load<T, V, K>(a, x, g.ldx, g, s);
+    slab_load<T, V, K>(d, dy, g.ldd, g, s);
+    if constexpr (RES && kAct) slab_load<T, V, K>(e, res, g.ldr, g, s);
+    const double mean = stats[2 * id], rstd = stats[2 * id + 1];
+    const float mh = (float)mean, ml = (float)(mean - (double)mh), rs = (float)rstd;
+    Coef<V> cf;
+    float wc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int ch = s.chunk * V + i;
+        wc[i] = s.on && w ? w[ch] : 1.f;
+        coef_of(cf, i, mean, rstd, (double)wc[i], s.on && b ? (double)b[ch] : 0.0);
+    }
+    auto gradient = [&](int k, int i) {                   // dz
+        float dz = to_f(d[k].v[i]);
+        if constexpr (kAct) {
+            float z = affine(to_f(a[k].v[i]), cf.ah[i], cf.al[i], cf.bh[i], cf.bl[i]);
+            if constexpr (RES) z += to_f(e[k].v[i]);
+            dz = act_bwd<ACT, kExact>(dz, z);
+        }
+        return dz;
+    };
+    float acc[2 * V];
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (s.on && s.row + (long)k * s.rows < g.hw)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float dz = gradient(k, i);
+                acc[i] += dz;
+                acc[V + i] = fmaf(dz, xhat_of(to_f(a[k].v[i]), mh, ml, rs), acc[V + i]);
+            }
+    join_rows<2 * V, kBlock>(acc, lds, g.cv, s.rows, s.row);
+    double t1 = 0.0, t2 = 0.0;
+    if (s.row == 0) {
+        float* o = part + s.n * 2 * g.C + (long)s.chunk * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            o[i] = acc[i];
+            o[g.C + i] = acc[V + i];
+            t1 += (double)wc[i] * (double)acc[i];
+            t2 += (double)wc[i] * (double)acc[V + i];
+        }
+    }
+    const double inv = 1.0 / ((double)g.hw * g.cpg);
+    const float m1 = (float)(block_sum(t1, sums) * inv), m2 = (float)(block_sum(t2, sums) * inv);
+    if (!s.on) return;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long r = s.row + (long)k * s.rows;
+        if (r < g.hw) {
+            float f[V], h[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                h[i] = gradient(k, i);
+                const float t = __fmul_rn(wc[i], h[i]) - m1;
+                f[i] = rs * fmaf(-xhat_of(to_f(a[k].v[i]), mh, ml, rs), m2, t);
+            }
+            const long at = (s.n * g.hw + r) * g.C + (long)s.chunk * V;
+            store_pack<T, V>(dx + at, f);
+            if constexpr (RES && kAct) store_pack<T, V>(dres + at, h);
+        }
+    }
+}
+
+// packs per thread that hold a group (0: it does not fit, or its packs would straddle groups)
+int slab_packs(const Geo& g, int V, int most) {
+    if (V == 1 || g.cpg % V || g.cpg / V > kBlock || g.hw > (long)most * kBlock) return 0;
+    const long rows = kBlock / (g.cpg / V), n = (g.hw + rows - 1) / rows;
+    return n <= 4 ? 4 : n <= most ? kHeld : 0;
+}
+
+Geo make_slab(Geo g, int V) {
+    g.cv = g.cpg / V;
+    g.splits = 1;
+    return g;
+}
+
 Geo make_geo(long images, long hw, int C, int G, int V, float eps, long ldx, long ldr, long ldd) {
     Geo g;
     g.hw = hw; g.C = C; g.G = G; g.cpg = C / G; g.eps = eps;
@@ -422,9 +651,9 @@ Geo make_geo(long images, long hw, int C, int G, int V, float eps, long ldx, lon
     g.cblocks = (g.cv + 255) / 256;
     g.cb = (g.cv + g.cblocks - 1) / g.cblocks;
     g.rpp = 256 / g.cb;
-    // about 2048 blocks in all (eight to a CU), and no range shorter than two unrolled steps of the block's rows
+    // about 1024 blocks in all (four to a CU), and no range shorter than two unrolled steps of the block's rows
     const long per = (long)images * g.cblocks;
-    long splits = (2048 + per - 1) / per;
+    long splits = (1024 + per - 1) / per;
     const long most = (hw + (long)g.rpp * kUnroll * 2 - 1) / ((long)g.rpp * kUnroll * 2);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
@@ -433,6 +662,11 @@ Geo make_geo(long images, long hw, int C, int G, int V, float eps, long ldx, lon
     g.ldx = ldx; g.ldr = ldr; g.ldd = ldd;
     return g;
 }
+
+// waves of a team: four where a group has more than a wave's worth of items
+int team_width(const Geo& g) { return (long)g.cpg * g.splits > 64 ? 4 : 1; }
+
+dim3 team_grid(long groups, int wide) { return dim3((unsigned)(wide == 4 ? groups : (groups + 3) / 4)); }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -456,12 +690,23 @@ struct Fwd {
 
 template <typename T, int V, int ACT, bool RES>
 int run_fwd(const Geo& g, long images, const Fwd& f) {
-    const long blocks = images * g.cblocks * g.splits, waves = images * g.G;
-    if (blocks > 0x7fffffffL || (waves + 3) / 4 > 0x7fffffffL) return -3;
+    const long blocks = images * g.cblocks * g.splits, groups = images * g.G;
+    const int wide = team_width(g);
+    if (blocks > 0x7fffffffL || groups > 0x7fffffffL) return -3;
+    if constexpr (V > 1) {
+        const int held = slab_packs(g, V, kHeld);
+        const Geo sg = make_slab(g, V);
+        const dim3 grid((unsigned)groups);
+        const T *x = (const T*)f.x, *r = (const T*)f.res;
+        if (held == 4) gn_slab_fwd_kernel<T, V, ACT, RES, 4><<<grid, kBlock, 0, f.stream>>>(sg, x, r, f.w, f.b, (T*)f.y, f.stats);
+        if (held == kHeld)
+            gn_slab_fwd_kernel<T, V, ACT, RES, kHeld><<<grid, kBlock, 0, f.stream>>>(sg, x, r, f.w, f.b, (T*)f.y, f.stats);
+        if (held) return DP_LAUNCH_STATUS();
+    }
     float* pivot = f.ws;
     float* part = f.ws + images * g.C;
     gn_stats_kernel<T, V><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, part, pivot);
-    gn_finish_kernel<<<dim3((unsigned)((waves + 3) / 4)), 256, 0, f.stream>>>(g, waves, part, pivot, f.stats);
+    gn_finish_kernel<<<team_grid(groups, wide), 256, 0, f.stream>>>(g, groups, wide, part, pivot, f.stats);
     gn_apply_kernel<T, V, ACT, RES><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, (const T*)f.res, f.w, f.b,
                                                                                 f.stats, (T*)f.y);
     return DP_LAUNCH_STATUS();
@@ -474,14 +719,32 @@ struct Bwd {
 
 template <typename T, int V, int ACT, bool RES>
 int run_bwd(const Geo& g, long images, const Bwd& f) {
-    const long blocks = images * g.cblocks * g.splits, gblocks = (images * g.G + 3) / 4;
-    if (blocks > 0x7fffffffL || gblocks + g.C > 0x7fffffffL) return -3;
+    const long blocks = images * g.cblocks * g.splits, groups = images * g.G;
+    const int wide = team_width(g);
+    if (blocks > 0x7fffffffL || groups > 0x7fffffffL) return -3;
+    if constexpr (V > 1) {
+        constexpr int kMost = RES && ACT != kNone ? kHeld / 2 : kHeld;      // (a third operand to hold)
+        const int held = slab_packs(g, V, kMost);
+        const Geo sg = make_slab(g, V);
+        const dim3 grid((unsigned)groups);
+        const T *dy = (const T*)f.dy, *x = (const T*)f.x, *r = (const T*)f.res;
+        if (held == 4)
+            gn_slab_bwd_kernel<T, V, ACT, RES, 4><<<grid, kBlock, 0, f.stream>>>(sg, dy, x, r, f.w, f.b, f.stats, (T*)f.dx,
+                                                                              (T*)f.dres, f.ws);
+        if (held == kHeld)
+            gn_slab_bwd_kernel<T, V, ACT, RES, kMost><<<grid, kBlock, 0, f.stream>>>(sg, dy, x, r, f.w, f.b, f.stats,
+                                                                                  (T*)f.dx, (T*)f.dres, f.ws);
+        if (held && (f.dw || f.db))
+            gn_bwd_params_kernel<<<dim3((unsigned)((g.C + 15) / 16)), 1024, 0, f.stream>>>(g.C, images, f.ws, f.dw, f.db);
+        if (held) return DP_LAUNCH_STATUS();
+    }
     float* means = f.ws;
     float* part = f.ws + 2 * images * g.G;
     gn_bwd_reduce_kernel<T, V, ACT, RES><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, part);
-    gn_bwd_finish_kernel<<<dim3((unsigned)(gblocks + (g.C + 255) / 256)), 256, 0, f.stream>>>(
-        g, images, (int)gblocks, part, f.w, means, f.dw, f.db);
+    gn_bwd_means_kernel<<<team_grid(groups, wide), 256, 0, f.stream>>>(g, groups, wide, part, f.w, means);
+    if (f.dw || f.db)
+        gn_bwd_params_kernel<<<dim3((unsigned)((g.C + 15) / 16)), 1024, 0, f.stream>>>(g.C, images * g.splits, part, f.dw, f.db);
     gn_bwd_apply_kernel<T, V, ACT, RES><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, means, (T*)f.dx, (T*)f.dres);
     return DP_LAUNCH_STATUS();
