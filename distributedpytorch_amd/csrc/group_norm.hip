@@ -34,20 +34,30 @@ template <> __device__ __forceinline__ bf16_raw from_f<bf16_raw>(float v) { retu
 template <> __device__ __forceinline__ f16 from_f<f16>(float v) { return (f16)v; }
 
 // V elements of 16 bytes in all (V > 1) or a single one
-template <typename T, int V> struct Pack { T v[V]; };
-template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
-    Pack<T, V> r;
-    if constexpr (V == 1) r.v[0] = *p;
-    else { static_assert(sizeof(T) * V == 16, "one 16-byte access"); r = __builtin_bit_cast(Pack<T, V>, *reinterpret_cast<const uint4*>(p)); }
-    return r;
-}
-template <typename T, int V> __device__ __forceinline__ void store_pack(T* p, const float* f) {
-    Pack<T, V> r;
+template <typename T, int V> struct Pack {
+    uint4 raw;
+    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ float get(int i) const {
+        const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (__is_same(T, bf16_raw)) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+        else return (float)__builtin_bit_cast(f16, (unsigned short)(w[i >> 1] >> (i & 1 ? 16 : 0)));
+    }
+    static __device__ __forceinline__ void store(T* p, const float* f) {
+        T t[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = from_f<T>(f[i]);
-    if constexpr (V == 1) *p = r.v[0];
-    else *reinterpret_cast<uint4*>(p) = __builtin_bit_cast(uint4, r);
-}
+        for (int i = 0; i < V; ++i) t[i] = from_f<T>(f[i]);
+        uint4 u;
+        __builtin_memcpy(&u, t, 16);
+        *reinterpret_cast<uint4*>(p) = u;
+    }
+};
+template <typename T> struct Pack<T, 1> {
+    T one;
+    __device__ __forceinline__ void load(const T* p) { one = *p; }
+    __device__ __forceinline__ float get(int) const { return to_f(one); }
+    static __device__ __forceinline__ void store(T* p, const float* f) { *p = from_f<T>(f[0]); }
+};
 
 // A block of 256 threads: cb neighbouring packs of a row by rpp rows; a thread keeps its channels and walks down rows.
 struct Geo {
@@ -62,9 +72,8 @@ struct Geo {
 
 struct Place { long n, row, row_end; int chunk, split, lane_row; bool on; };
 
-__device__ __forceinline__ Place place(const Geo& g) {
+__device__ __forceinline__ Place place(const Geo& g, long id) {
     Place p;
-    const long id = blockIdx.x;
     p.split = (int)(id % g.splits);
     const long t = id / g.splits;
     const int cblk = (int)(t % g.cblocks);
@@ -97,11 +106,24 @@ template <int K, int N> __device__ __forceinline__ void join_rows(float* acc, fl
 
 constexpr int kUnroll = 4;   // packs in flight per thread and operand
 
+// body(u, row) for the thread's rows: fetch(u, row) of kUnroll rows first, so that their loads are in flight together
+template <typename F, typename B> __device__ __forceinline__ void walk(const Geo& g, const Place& p, F fetch, B body) {
+    long r = p.row;
+    const long step = g.rpp;
+    for (; r + (kUnroll - 1) * step < p.row_end; r += kUnroll * step) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) fetch(u, r + u * step);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) body(u, r + u * step);
+    }
+    for (; r < p.row_end; r += step) { fetch(0, r); body(0, r); }
+}
+
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gn_stats_kernel(Geo g, const T* __restrict__ x, float* __restrict__ part,
                                                        float* __restrict__ pivot) {
     __shared__ float lds[2 * V * 256];
-    const Place p = place(g);
+    const Place p = place(g, blockIdx.x);
     float acc[2 * V];
 #pragma unroll
     for (int k = 0; k < 2 * V; ++k) acc[k] = 0.f;
@@ -112,28 +134,24 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(Geo g, const T* __restric
         for (int i = 0; i < V; ++i) pv[i] = 0.f;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const Pack<T, V> a = load_pack<T, V>(base + (g.hw * s / 4) * g.ldx);
+            Pack<T, V> a;
+            a.load(base + (g.hw * s / 4) * g.ldx);
 #pragma unroll
-            for (int i = 0; i < V; ++i) pv[i] += 0.25f * to_f(a.v[i]);
+            for (int i = 0; i < V; ++i) pv[i] += 0.25f * a.get(i);
         }
         if (p.split == 0 && p.lane_row == 0)
 #pragma unroll
             for (int i = 0; i < V; ++i) pivot[p.n * g.C + (long)p.chunk * V + i] = pv[i];
-        for (long r = p.row; r < p.row_end; r += (long)kUnroll * g.rpp) {
-            Pack<T, V> a[kUnroll];
+        Pack<T, V> a[kUnroll];
+        walk(g, p, [&](int u, long r) { a[u].load(base + r * g.ldx); },
+             [&](int u, long) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * g.rpp < p.row_end) a[u] = load_pack<T, V>(base + (r + u * g.rpp) * g.ldx);
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * g.rpp < p.row_end)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float d = to_f(a[u].v[i]) - pv[i];
-                        acc[i] += d;
-                        acc[V + i] = fmaf(d, d, acc[V + i]);
-                    }
-        }
+                 for (int i = 0; i < V; ++i) {
+                     const float d = a[u].get(i) - pv[i];
+                     acc[i] += d;
+                     acc[V + i] = fmaf(d, d, acc[V + i]);
+                 }
+             });
     }
     join_rows<2 * V, 256>(acc, lds, g.cb, g.rpp, p.lane_row);
     if (p.on && p.lane_row == 0) {
@@ -209,31 +227,51 @@ __global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int 
     }
 }
 
-// per-channel constants of one thread
-template <int V> struct Coef { float ah[V], al[V], bh[V], bl[V]; };        // z = x a + b (+ residual)
+// Constants of one thread's V channels; S: how many groups its pack can touch (1: cpg is a multiple of V, else V).
+template <int V, int S> struct Norm { float mh[S], ml[S], rs[S]; double mean[S], rstd[S]; };   // xhat = (x - mean) rstd
 
-template <int V>
-__device__ __forceinline__ void coef_of(Coef<V>& c, int i, double mean, double rstd, double w, double b) {
-    const double a = w * rstd, bb = b - mean * a;
-    c.ah[i] = (float)a; c.al[i] = (float)(a - (double)c.ah[i]);
-    c.bh[i] = (float)bb; c.bl[i] = (float)(bb - (double)c.bh[i]);
-}
-
-template <int V>
-__device__ __forceinline__ Coef<V> coef(const Geo& g, const Place& p, const double* stats, const float* w, const float* b) {
-    Coef<V> c;
+template <int V, int S>
+__device__ __forceinline__ Norm<V, S> norm_of(const Geo& g, const Place& p, const double* stats) {
+    Norm<V, S> c;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int ch = p.chunk * V + i;
-        const double* st = stats + 2 * (p.n * g.G + ch / g.cpg);
-        coef_of(c, i, st[0], st[1], w ? (double)w[ch] : 1.0, b ? (double)b[ch] : 0.0);
+    for (int i = 0; i < S; ++i) {
+        const double* st = stats + 2 * (p.n * g.G + (p.chunk * V + i) / g.cpg);
+        c.mean[i] = st[0]; c.rstd[i] = st[1];
+        c.mh[i] = (float)st[0]; c.ml[i] = (float)(st[0] - (double)c.mh[i]); c.rs[i] = (float)st[1];
     }
     return c;
 }
 
-// Near z = 0 the first product leaves z almost exactly and the second adds what the rounded coefficients left out.
-__device__ __forceinline__ float affine(float x, float ah, float al, float bh, float bl) {
-    return fmaf(x, ah, bh) + fmaf(x, al, bl);
+// z from x or from d = x - mh.  With ReLU the sign of z decides whole gradients: there z = x a + b with a and b split
+// into a rounded value and its remainder (near z = 0 the first product leaves z almost exactly, and the second adds what
+// the rounded coefficients left out).  Elsewhere z = d a + b', whose error is a few 2^-24 of |d a| and |b'|.
+template <int V, bool SPLIT> struct Coef {
+    float ah[V], bh[V], al[SPLIT ? V : 1], bl[SPLIT ? V : 1];
+    template <int S>
+    __device__ __forceinline__ void set(int i, const Norm<V, S>& n, float w, float b) {
+        const double a = (double)w * n.rstd[i % S];
+        ah[i] = (float)a;
+        if constexpr (SPLIT) {
+            const double bb = (double)b - n.mean[i % S] * a;
+            bh[i] = (float)bb;
+            al[i] = (float)(a - (double)ah[i]);
+            bl[i] = (float)(bb - (double)bh[i]);
+        } else {
+            bh[i] = (float)((double)b - (n.mean[i % S] - (double)n.mh[i % S]) * a);
+        }
+    }
+    __device__ __forceinline__ float z(int i, float x, float d) const {
+        if constexpr (SPLIT) return fmaf(x, ah[i], bh[i]) + fmaf(x, al[i], bl[i]);
+        else return fmaf(d, ah[i], bh[i]);
+    }
+};
+
+template <int V, int S, bool SPLIT>
+__device__ __forceinline__ Coef<V, SPLIT> coef_of(const Norm<V, S>& n, int chunk, bool on, const float* w, const float* b) {
+    Coef<V, SPLIT> c;
+#pragma unroll
+    for (int i = 0; i < V; ++i) c.set(i, n, on && w ? w[chunk * V + i] : 1.f, on && b ? b[chunk * V + i] : 0.f);
+    return c;
 }
 
 template <bool EXACT> __device__ __forceinline__ float sigmoid(float z) {
@@ -254,105 +292,83 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float act_bwd(float dy
     else return dy;
 }
 
-template <typename T, int V, int ACT, bool RES>
+// The element passes take the blocks in reverse: the last level of cache still holds what the pass before read last.
+template <typename T, int V, int S, int ACT, bool RES>
 __global__ __launch_bounds__(256) void gn_apply_kernel(Geo g, const T* __restrict__ x, const T* __restrict__ res,
                                                        const float* __restrict__ w, const float* __restrict__ b,
                                                        const double* __restrict__ stats, T* __restrict__ y) {
     constexpr bool kExact = sizeof(T) == 4;
-    const Place p = place(g);
+    const Place p = place(g, (long)gridDim.x - 1 - blockIdx.x);
     if (!p.on) return;
-    const Coef<V> cf = coef<V>(g, p, stats, w, b);
+    const Norm<V, S> nc = norm_of<V, S>(g, p, stats);
+    const Coef<V, ACT == kRelu> cf = coef_of<V, S, ACT == kRelu>(nc, p.chunk, true, w, b);
     const long col = (long)p.chunk * V, row0 = p.n * g.hw;
-    for (long r = p.row; r < p.row_end; r += (long)kUnroll * g.rpp) {
-        Pack<T, V> a[kUnroll], e[kUnroll];
+    const T *xb = x + row0 * g.ldx + col, *rb = RES ? res + row0 * g.ldr + col : nullptr;
+    T* yb = y + row0 * g.C + col;
+    Pack<T, V> a[kUnroll], e[kUnroll];
+    walk(g, p,
+         [&](int u, long r) {
+             a[u].load(xb + r * g.ldx);
+             if constexpr (RES) e[u].load(rb + r * g.ldr);
+         },
+         [&](int u, long r) {
+             float f[V];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const long q = r + u * g.rpp;
-            if (q < p.row_end) {
-                a[u] = load_pack<T, V>(x + (row0 + q) * g.ldx + col);
-                if constexpr (RES) e[u] = load_pack<T, V>(res + (row0 + q) * g.ldr + col);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const long q = r + u * g.rpp;
-            if (q < p.row_end) {
-                float f[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float z = affine(to_f(a[u].v[i]), cf.ah[i], cf.al[i], cf.bh[i], cf.bl[i]);
-                    if constexpr (RES) z += to_f(e[u].v[i]);
-                    f[i] = act_fwd<ACT, kExact>(z);
-                }
-                store_pack<T, V>(y + (row0 + q) * g.C + col, f);
-            }
-        }
-    }
+             for (int i = 0; i < V; ++i) {
+                 const float xv = a[u].get(i);
+                 float z = cf.z(i, xv, xv - nc.mh[i % S]);
+                 if constexpr (RES) z += e[u].get(i);
+                 f[i] = act_fwd<ACT, kExact>(z);
+             }
+             Pack<T, V>::store(yb + r * g.C, f);
+         });
 }
-
-template <int V> struct Norm { float mh[V], ml[V], rs[V]; };               // xhat = (x - mean) rstd
-
-template <int V> __device__ __forceinline__ Norm<V> norm_coef(const Geo& g, const Place& p, const double* stats) {
-    Norm<V> c;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const double* st = stats + 2 * (p.n * g.G + (p.chunk * V + i) / g.cpg);
-        c.mh[i] = (float)st[0]; c.ml[i] = (float)(st[0] - (double)c.mh[i]); c.rs[i] = (float)st[1];
-    }
-    return c;
-}
-
-__device__ __forceinline__ float xhat_of(float x, float mh, float ml, float rs) { return ((x - mh) - ml) * rs; }
 
 // part[n, split, 0 | 1, c] = sum dz | sum dz xhat over the rows of the split
-template <typename T, int V, int ACT, bool RES>
+template <typename T, int V, int S, int ACT, bool RES>
 __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __restrict__ dy, const T* __restrict__ x,
                                                             const T* __restrict__ res, const float* __restrict__ w,
                                                             const float* __restrict__ b,
                                                             const double* __restrict__ stats, float* __restrict__ part) {
-    constexpr bool kExact = sizeof(T) == 4;
+    constexpr bool kExact = sizeof(T) == 4, kRes = RES && ACT != kNone;
     __shared__ float lds[2 * V * 256];
-    const Place p = place(g);
-    float acc[2 * V];
+    const Place p = place(g, blockIdx.x);
+    float acc[2 * V];                        // sum dz | sum dz (x - mh): the rest of xhat is put in at the end
 #pragma unroll
     for (int k = 0; k < 2 * V; ++k) acc[k] = 0.f;
+    Norm<V, S> nc;
     if (p.on) {
-        const Coef<V> cf = coef<V>(g, p, stats, w, b);
-        const Norm<V> nc = norm_coef<V>(g, p, stats);
+        nc = norm_of<V, S>(g, p, stats);
+        const Coef<V, ACT == kRelu> cf = coef_of<V, S, ACT == kRelu>(nc, p.chunk, true, w, b);
         const long col = (long)p.chunk * V, row0 = p.n * g.hw;
-        for (long r = p.row; r < p.row_end; r += (long)kUnroll * g.rpp) {
-            Pack<T, V> a[kUnroll], d[kUnroll], e[kUnroll];
+        const T *xb = x + row0 * g.ldx + col, *db = dy + row0 * g.ldd + col, *rb = kRes ? res + row0 * g.ldr + col : nullptr;
+        Pack<T, V> a[kUnroll], d[kUnroll], e[kUnroll];
+        walk(g, p,
+             [&](int u, long r) {
+                 a[u].load(xb + r * g.ldx);
+                 d[u].load(db + r * g.ldd);
+                 if constexpr (kRes) e[u].load(rb + r * g.ldr);
+             },
+             [&](int u, long) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const long q = r + u * g.rpp;
-                if (q < p.row_end) {
-                    a[u] = load_pack<T, V>(x + (row0 + q) * g.ldx + col);
-                    d[u] = load_pack<T, V>(dy + (row0 + q) * g.ldd + col);
-                    if constexpr (RES && ACT != kNone) e[u] = load_pack<T, V>(res + (row0 + q) * g.ldr + col);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (r + u * g.rpp < p.row_end)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float xv = to_f(a[u].v[i]);
-                        float dz = to_f(d[u].v[i]);
-                        if constexpr (ACT != kNone) {
-                            float z = affine(xv, cf.ah[i], cf.al[i], cf.bh[i], cf.bl[i]);
-                            if constexpr (RES) z += to_f(e[u].v[i]);
-                            dz = act_bwd<ACT, kExact>(dz, z);
-                        }
-                        acc[i] += dz;
-                        acc[V + i] = fmaf(dz, xhat_of(xv, nc.mh[i], nc.ml[i], nc.rs[i]), acc[V + i]);
-                    }
-        }
+                 for (int i = 0; i < V; ++i) {
+                     const float xv = a[u].get(i), xd = xv - nc.mh[i % S];
+                     float dz = d[u].get(i);
+                     if constexpr (ACT != kNone) {
+                         float z = cf.z(i, xv, xd);
+                         if constexpr (kRes) z += e[u].get(i);
+                         dz = act_bwd<ACT, kExact>(dz, z);
+                     }
+                     acc[i] += dz;
+                     acc[V + i] = fmaf(dz, xd, acc[V + i]);
+                 }
+             });
     }
     join_rows<2 * V, 256>(acc, lds, g.cb, g.rpp, p.lane_row);
     if (p.on && p.lane_row == 0) {
         float* o = part + ((p.n * g.splits + p.split) * 2) * g.C + (long)p.chunk * V;
 #pragma unroll
-        for (int i = 0; i < V; ++i) { o[i] = acc[i]; o[g.C + i] = acc[V + i]; }
+        for (int i = 0; i < V; ++i) { o[i] = acc[i]; o[g.C + i] = fmaf(-nc.ml[i % S], acc[i], acc[V + i]) * nc.rs[i % S]; }
     }
 }
 
@@ -400,67 +416,62 @@ __global__ __launch_bounds__(1024) void gn_bwd_params_kernel(int C, long lines, 
     }
 }
 
-template <typename T, int V, int ACT, bool RES>
+template <typename T, int V, int S, int ACT, bool RES>
 __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __restrict__ dy, const T* __restrict__ x,
                                                            const T* __restrict__ res, const float* __restrict__ w,
                                                            const float* __restrict__ b, const double* __restrict__ stats,
                                                            const float* __restrict__ means, T* __restrict__ dx,
                                                            T* __restrict__ dres) {
-    constexpr bool kExact = sizeof(T) == 4;
-    const Place p = place(g);
+    constexpr bool kExact = sizeof(T) == 4, kRes = RES && ACT != kNone;
+    const Place p = place(g, (long)gridDim.x - 1 - blockIdx.x);
     if (!p.on) return;
-    const Coef<V> cf = coef<V>(g, p, stats, w, b);
-    const Norm<V> nc = norm_coef<V>(g, p, stats);
-    float wc[V], m1[V], m2[V];
+    const Norm<V, S> nc = norm_of<V, S>(g, p, stats);
+    const Coef<V, ACT == kRelu> cf = coef_of<V, S, ACT == kRelu>(nc, p.chunk, true, w, b);
+    float wc[V], m1[S], k2[S];               // dx = rs ((w dz - m1) - (x - mh) k2)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int ch = p.chunk * V + i;
-        const float* m = means + 2 * (p.n * g.G + ch / g.cpg);
-        wc[i] = w ? w[ch] : 1.f; m1[i] = m[0]; m2[i] = m[1];
+    for (int i = 0; i < V; ++i) wc[i] = w ? w[p.chunk * V + i] : 1.f;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        const float* m = means + 2 * (p.n * g.G + (p.chunk * V + i) / g.cpg);
+        k2[i] = nc.rs[i] * m[1];
+        m1[i] = fmaf(-nc.ml[i], k2[i], m[0]);
     }
     const long col = (long)p.chunk * V, row0 = p.n * g.hw;
-    for (long r = p.row; r < p.row_end; r += (long)kUnroll * g.rpp) {
-        Pack<T, V> a[kUnroll], d[kUnroll], e[kUnroll];
+    const T *xb = x + row0 * g.ldx + col, *db = dy + row0 * g.ldd + col, *rb = kRes ? res + row0 * g.ldr + col : nullptr;
+    T *ob = dx + row0 * g.C + col, *hb = kRes ? dres + row0 * g.C + col : nullptr;
+    Pack<T, V> a[kUnroll], d[kUnroll], e[kUnroll];
+    walk(g, p,
+         [&](int u, long r) {
+             a[u].load(xb + r * g.ldx);
+             d[u].load(db + r * g.ldd);
+             if constexpr (kRes) e[u].load(rb + r * g.ldr);
+         },
+         [&](int u, long r) {
+             float f[V], h[V];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const long q = r + u * g.rpp;
-            if (q < p.row_end) {
-                a[u] = load_pack<T, V>(x + (row0 + q) * g.ldx + col);
-                d[u] = load_pack<T, V>(dy + (row0 + q) * g.ldd + col);
-                if constexpr (RES && ACT != kNone) e[u] = load_pack<T, V>(res + (row0 + q) * g.ldr + col);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const long q = r + u * g.rpp;
-            if (q < p.row_end) {
-                float f[V], h[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float xv = to_f(a[u].v[i]);
-                    float dz = to_f(d[u].v[i]);
-                    if constexpr (ACT != kNone) {
-                        float z = affine(xv, cf.ah[i], cf.al[i], cf.bh[i], cf.bl[i]);
-                        if constexpr (RES) z += to_f(e[u].v[i]);
-                        dz = act_bwd<ACT, kExact>(dz, z);
-                    }
-                    h[i] = dz;
-                    // w dz rounded by itself: in a group of one element it then equals m1 and the gradient is zero
-                    const float t = __fmul_rn(wc[i], dz) - m1[i];
-                    f[i] = nc.rs[i] * fmaf(-xhat_of(xv, nc.mh[i], nc.ml[i], nc.rs[i]), m2[i], t);
-                }
-                store_pack<T, V>(dx + (row0 + q) * g.C + col, f);
-                if constexpr (RES && ACT != kNone) store_pack<T, V>(dres + (row0 + q) * g.C + col, h);
-            }
-        }
-    }
+             for (int i = 0; i < V; ++i) {
+                 const float xv = a[u].get(i), xd = xv - nc.mh[i % S];
+                 float dz = d[u].get(i);
+                 if constexpr (ACT != kNone) {
+                     float z = cf.z(i, xv, xd);
+                     if constexpr (kRes) z += e[u].get(i);
+                     dz = act_bwd<ACT, kExact>(dz, z);
+                 }
+                 h[i] = dz;
+                 // w dz rounded by itself: in a group of one element it then equals m1 and the gradient is zero
+                 const float t = __fmul_rn(wc[i], dz) - m1[i % S];
+                 f[i] = nc.rs[i % S] * fmaf(-xd, k2[i % S], t);
+             }
+             Pack<T, V>::store(ob + r * g.C, f);
+             if constexpr (kRes) Pack<T, V>::store(hb + r * g.C, h);
+         });
 }
 
 // ------------------------------------------------------------------------------------------------ groups that fit a block
-// Where a group's map fits the registers of one block (at most kHeld packs for each of its 512 threads), the block reads
+// Where a group's map fits the registers of one block (at most 4 packs for each of its 512 threads), the block reads
 // it once, takes the statistics from its registers (the mean first, then the squared differences from it) and writes the
 // result: one launch forward, and no second read.  Needs whole packs inside a group (cpg a multiple of V).
-constexpr int kBlock = 512, kHeld = 16;
+constexpr int kBlock = 512, kHeld = 4;
 
 struct Slab { long n; int chunk, row, rows; bool on; };
 
@@ -491,15 +502,16 @@ __device__ __forceinline__ void slab_load(Pack<T, V> (&a)[K], const T* base, lon
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const long r = s.row + (long)k * s.rows;
-        if (s.on && r < g.hw) a[k] = load_pack<T, V>(base + (s.n * g.hw + r) * ld + (long)s.chunk * V);
+        if (s.on && r < g.hw) a[k].load(base + (s.n * g.hw + r) * ld + (long)s.chunk * V);
     }
 }
 
-template <typename T, int V, int ACT, bool RES, int K>
+template <typename T, int V, int ACT, bool RES>
 __global__ __launch_bounds__(kBlock) void gn_slab_fwd_kernel(Geo g, const T* __restrict__ x, const T* __restrict__ res,
                                                              const float* __restrict__ w, const float* __restrict__ b,
                                                              T* __restrict__ y, double* __restrict__ stats) {
     constexpr bool kExact = sizeof(T) == 4;
+    constexpr int K = kHeld;
     __shared__ double lds[kBlock / 64];
     const long id = blockIdx.x;
     const Slab s = slab_of(g, id);
@@ -508,7 +520,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_fwd_kernel(Geo g, const T* __r
     if constexpr (RES) slab_load<T, V, K>(e, res, g.ldr, g, s);
     const double inv = 1.0 / ((double)g.hw * g.cpg);
     // differences from the thread's own first element, so that a mean far above the spread costs no bits
-    const float first = s.on && s.row < g.hw ? to_f(a[0].v[0]) : 0.f;
+    const float first = s.on && s.row < g.hw ? a[0].get(0) : 0.f;
     float sum = 0.f;
     int held = 0;
 #pragma unroll
@@ -516,25 +528,24 @@ __global__ __launch_bounds__(kBlock) void gn_slab_fwd_kernel(Geo g, const T* __r
         if (s.on && s.row + (long)k * s.rows < g.hw) {
             held += V;
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum += to_f(a[k].v[i]) - first;
+            for (int i = 0; i < V; ++i) sum += a[k].get(i) - first;
         }
     const double mean = block_sum((double)sum + (double)held * (double)first, lds) * inv;
-    const float mh = (float)mean, ml = (float)(mean - (double)mh);
+    Norm<V, 1> nc;
+    nc.mean[0] = mean;
+    nc.mh[0] = (float)mean;
+    nc.ml[0] = (float)(mean - (double)nc.mh[0]);
     float sq = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
         if (s.on && s.row + (long)k * s.rows < g.hw)
 #pragma unroll
-            for (int i = 0; i < V; ++i) { const float d = (to_f(a[k].v[i]) - mh) - ml; sq = fmaf(d, d, sq); }
+            for (int i = 0; i < V; ++i) { const float d = (a[k].get(i) - nc.mh[0]) - nc.ml[0]; sq = fmaf(d, d, sq); }
     const double rstd = 1.0 / sqrt(block_sum((double)sq, lds) * inv + (double)g.eps);
     if (threadIdx.x == 0) { stats[2 * id] = mean; stats[2 * id + 1] = rstd; }
     if (!s.on) return;
-    Coef<V> cf;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int ch = s.chunk * V + i;
-        coef_of(cf, i, mean, rstd, w ? (double)w[ch] : 1.0, b ? (double)b[ch] : 0.0);
-    }
+    nc.rstd[0] = rstd;
+    const Coef<V, ACT == kRelu> cf = coef_of<V, 1, ACT == kRelu>(nc, s.chunk, true, w, b);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const long r = s.row + (long)k * s.rows;
@@ -542,23 +553,25 @@ __global__ __launch_bounds__(kBlock) void gn_slab_fwd_kernel(Geo g, const T* __r
             float f[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float z = affine(to_f(a[k].v[i]), cf.ah[i], cf.al[i], cf.bh[i], cf.bl[i]);
-                if constexpr (RES) z += to_f(e[k].v[i]);
+                const float xv = a[k].get(i);
+                float z = cf.z(i, xv, xv - nc.mh[0]);
+                if constexpr (RES) z += e[k].get(i);
                 f[i] = act_fwd<ACT, kExact>(z);
             }
-            store_pack<T, V>(y + (s.n * g.hw + r) * g.C + (long)s.chunk * V, f);
+            Pack<T, V>::store(y + (s.n * g.hw + r) * g.C + (long)s.chunk * V, f);
         }
     }
 }
 
 // part[n, 0 | 1, c] = sum dz | sum dz xhat of the image, for dw and db
-template <typename T, int V, int ACT, bool RES, int K>
+template <typename T, int V, int ACT, bool RES>
 __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __restrict__ dy, const T* __restrict__ x,
                                                              const T* __restrict__ res, const float* __restrict__ w,
                                                              const float* __restrict__ b,
                                                              const double* __restrict__ stats, T* __restrict__ dx,
                                                              T* __restrict__ dres, float* __restrict__ part) {
     constexpr bool kExact = sizeof(T) == 4, kAct = ACT != kNone;
+    constexpr int K = kHeld;
     __shared__ float lds[2 * V * kBlock];
     __shared__ double sums[kBlock / 64];
     const long id = blockIdx.x;
@@ -567,21 +580,20 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
     slab_load<T, V, K>(a, x, g.ldx, g, s);
     slab_load<T, V, K>(d, dy, g.ldd, g, s);
     if constexpr (RES && kAct) slab_load<T, V, K>(e, res, g.ldr, g, s);
-    const double mean = stats[2 * id], rstd = stats[2 * id + 1];
-    const float mh = (float)mean, ml = (float)(mean - (double)mh), rs = (float)rstd;
-    Coef<V> cf;
+    Norm<V, 1> nc;
+    nc.mean[0] = stats[2 * id];
+    nc.rstd[0] = stats[2 * id + 1];
+    nc.mh[0] = (float)nc.mean[0];
+    const float mh = nc.mh[0], ml = (float)(nc.mean[0] - (double)mh), rs = (float)nc.rstd[0];
+    const Coef<V, ACT == kRelu> cf = coef_of<V, 1, ACT == kRelu>(nc, s.chunk, s.on, w, b);
     float wc[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int ch = s.chunk * V + i;
-        wc[i] = s.on && w ? w[ch] : 1.f;
-        coef_of(cf, i, mean, rstd, (double)wc[i], s.on && b ? (double)b[ch] : 0.0);
-    }
-    auto gradient = [&](int k, int i) {                   // dz
-        float dz = to_f(d[k].v[i]);
+    for (int i = 0; i < V; ++i) wc[i] = s.on && w ? w[s.chunk * V + i] : 1.f;
+    auto gradient = [&](int k, int i, float xd) {         // dz
+        float dz = d[k].get(i);
         if constexpr (kAct) {
-            float z = affine(to_f(a[k].v[i]), cf.ah[i], cf.al[i], cf.bh[i], cf.bl[i]);
-            if constexpr (RES) z += to_f(e[k].v[i]);
+            float z = cf.z(i, a[k].get(i), xd);
+            if constexpr (RES) z += e[k].get(i);
             dz = act_bwd<ACT, kExact>(dz, z);
         }
         return dz;
@@ -594,9 +606,9 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
         if (s.on && s.row + (long)k * s.rows < g.hw)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float dz = gradient(k, i);
+                const float xd = a[k].get(i) - mh, dz = gradient(k, i, xd);
                 acc[i] += dz;
-                acc[V + i] = fmaf(dz, xhat_of(to_f(a[k].v[i]), mh, ml, rs), acc[V + i]);
+                acc[V + i] = fmaf(dz, xd, acc[V + i]);
             }
     join_rows<2 * V, kBlock>(acc, lds, g.cv, s.rows, s.row);
     double t1 = 0.0, t2 = 0.0;
@@ -604,6 +616,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
         float* o = part + s.n * 2 * g.C + (long)s.chunk * V;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+            acc[V + i] = fmaf(-ml, acc[i], acc[V + i]) * rs;
             o[i] = acc[i];
             o[g.C + i] = acc[V + i];
             t1 += (double)wc[i] * (double)acc[i];
@@ -611,7 +624,8 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
         }
     }
     const double inv = 1.0 / ((double)g.hw * g.cpg);
-    const float m1 = (float)(block_sum(t1, sums) * inv), m2 = (float)(block_sum(t2, sums) * inv);
+    const float mean1 = (float)(block_sum(t1, sums) * inv), k2 = rs * (float)(block_sum(t2, sums) * inv);
+    const float m1 = fmaf(-ml, k2, mean1);
     if (!s.on) return;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -620,22 +634,19 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
             float f[V], h[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                h[i] = gradient(k, i);
-                const float t = __fmul_rn(wc[i], h[i]) - m1;
-                f[i] = rs * fmaf(-xhat_of(to_f(a[k].v[i]), mh, ml, rs), m2, t);
+                const float xd = a[k].get(i) - mh;
+                h[i] = gradient(k, i, xd);
+                f[i] = rs * fmaf(-xd, k2, __fmul_rn(wc[i], h[i]) - m1);      // (as gn_bwd_apply_kernel)
             }
             const long at = (s.n * g.hw + r) * g.C + (long)s.chunk * V;
-            store_pack<T, V>(dx + at, f);
-            if constexpr (RES && kAct) store_pack<T, V>(dres + at, h);
+            Pack<T, V>::store(dx + at, f);
+            if constexpr (RES && kAct) Pack<T, V>::store(dres + at, h);
         }
     }
 }
 
-// packs per thread that hold a group (0: it does not fit, or its packs would straddle groups)
-int slab_packs(const Geo& g, int V, int most) {
-    if (V == 1 || g.cpg % V || g.cpg / V > kBlock || g.hw > (long)most * kBlock) return 0;
-    const long rows = kBlock / (g.cpg / V), n = (g.hw + rows - 1) / rows;
-    return n <= 4 ? 4 : n <= most ? kHeld : 0;
+bool fits_slab(const Geo& g, int V) {
+    return V > 1 && g.cpg % V == 0 && g.cpg / V <= kBlock && g.hw <= (long)kHeld * (kBlock / (g.cpg / V));
 }
 
 Geo make_slab(Geo g, int V) {
@@ -694,21 +705,18 @@ int run_fwd(const Geo& g, long images, const Fwd& f) {
     const int wide = team_width(g);
     if (blocks > 0x7fffffffL || groups > 0x7fffffffL) return -3;
     if constexpr (V > 1) {
-        const int held = slab_packs(g, V, kHeld);
-        const Geo sg = make_slab(g, V);
-        const dim3 grid((unsigned)groups);
-        const T *x = (const T*)f.x, *r = (const T*)f.res;
-        if (held == 4) gn_slab_fwd_kernel<T, V, ACT, RES, 4><<<grid, kBlock, 0, f.stream>>>(sg, x, r, f.w, f.b, (T*)f.y, f.stats);
-        if (held == kHeld)
-            gn_slab_fwd_kernel<T, V, ACT, RES, kHeld><<<grid, kBlock, 0, f.stream>>>(sg, x, r, f.w, f.b, (T*)f.y, f.stats);
-        if (held) return DP_LAUNCH_STATUS();
+        if (fits_slab(g, V)) {
+            gn_slab_fwd_kernel<T, V, ACT, RES><<<dim3((unsigned)groups), kBlock, 0, f.stream>>>(
+                make_slab(g, V), (const T*)f.x, (const T*)f.res, f.w, f.b, (T*)f.y, f.stats);
+            return DP_LAUNCH_STATUS();
+        }
     }
     float* pivot = f.ws;
     float* part = f.ws + images * g.C;
     gn_stats_kernel<T, V><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, part, pivot);
     gn_finish_kernel<<<team_grid(groups, wide), 256, 0, f.stream>>>(g, groups, wide, part, pivot, f.stats);
-    gn_apply_kernel<T, V, ACT, RES><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, (const T*)f.res, f.w, f.b,
-                                                                                f.stats, (T*)f.y);
+    const auto apply = g.cpg % V == 0 ? gn_apply_kernel<T, V, 1, ACT, RES> : gn_apply_kernel<T, V, V, ACT, RES>;
+    apply<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, (T*)f.y);
     return DP_LAUNCH_STATUS();
 }
 
@@ -723,29 +731,25 @@ int run_bwd(const Geo& g, long images, const Bwd& f) {
     const int wide = team_width(g);
     if (blocks > 0x7fffffffL || groups > 0x7fffffffL) return -3;
     if constexpr (V > 1) {
-        constexpr int kMost = RES && ACT != kNone ? kHeld / 2 : kHeld;      // (a third operand to hold)
-        const int held = slab_packs(g, V, kMost);
-        const Geo sg = make_slab(g, V);
-        const dim3 grid((unsigned)groups);
-        const T *dy = (const T*)f.dy, *x = (const T*)f.x, *r = (const T*)f.res;
-        if (held == 4)
-            gn_slab_bwd_kernel<T, V, ACT, RES, 4><<<grid, kBlock, 0, f.stream>>>(sg, dy, x, r, f.w, f.b, f.stats, (T*)f.dx,
-                                                                              (T*)f.dres, f.ws);
-        if (held == kHeld)
-            gn_slab_bwd_kernel<T, V, ACT, RES, kMost><<<grid, kBlock, 0, f.stream>>>(sg, dy, x, r, f.w, f.b, f.stats,
-                                                                                  (T*)f.dx, (T*)f.dres, f.ws);
-        if (held && (f.dw || f.db))
-            gn_bwd_params_kernel<<<dim3((unsigned)((g.C + 15) / 16)), 1024, 0, f.stream>>>(g.C, images, f.ws, f.dw, f.db);
-        if (held) return DP_LAUNCH_STATUS();
+        if (fits_slab(g, V)) {
+            gn_slab_bwd_kernel<T, V, ACT, RES><<<dim3((unsigned)groups), kBlock, 0, f.stream>>>(
+                make_slab(g, V), (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, (T*)f.dx, (T*)f.dres, f.ws);
+            if (f.dw || f.db)
+                gn_bwd_params_kernel<<<dim3((unsigned)((g.C + 15) / 16)), 1024, 0, f.stream>>>(g.C, images, f.ws, f.dw, f.db);
+            return DP_LAUNCH_STATUS();
+        }
     }
     float* means = f.ws;
     float* part = f.ws + 2 * images * g.G;
-    gn_bwd_reduce_kernel<T, V, ACT, RES><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
+    const bool one = g.cpg % V == 0;
+    const auto reduce = one ? gn_bwd_reduce_kernel<T, V, 1, ACT, RES> : gn_bwd_reduce_kernel<T, V, V, ACT, RES>;
+    const auto apply = one ? gn_bwd_apply_kernel<T, V, 1, ACT, RES> : gn_bwd_apply_kernel<T, V, V, ACT, RES>;
+    reduce<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, part);
     gn_bwd_means_kernel<<<team_grid(groups, wide), 256, 0, f.stream>>>(g, groups, wide, part, f.w, means);
     if (f.dw || f.db)
         gn_bwd_params_kernel<<<dim3((unsigned)((g.C + 15) / 16)), 1024, 0, f.stream>>>(g.C, images * g.splits, part, f.dw, f.db);
-    gn_bwd_apply_kernel<T, V, ACT, RES><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
+    apply<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, means, (T*)f.dx, (T*)f.dres);
     return DP_LAUNCH_STATUS();
 }
