@@ -13,7 +13,6 @@ Policy
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import sys
@@ -197,11 +196,19 @@ def stream_ptr() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def on_device(t: torch.Tensor):
-    """Context for a launch on ``t``'s own GPU (its current stream, its allocations), whichever GPU is current."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def launch(what: str, fn, t: torch.Tensor, *args) -> None:
+    """``fn(*args, stream)`` on the GPU of ``t`` and its current stream, whichever GPU is current; raises on a status.
+
+    Few Python steps on purpose: a backward pass runs in autograd's own thread, where every Python object that the
+    forward thread touched last is a cache miss (finding the stream through ``torch.cuda`` took 18 us there)."""
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != 0:
+        raise RuntimeError(f"HIP launcher '{what}' failed with status {status}")
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -8,6 +8,7 @@ plain torch operations.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -71,8 +72,13 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_floats(meta, backward) -> int:
+    return int(_lib().dp_xa_workspace(*meta, backward))
+
+
 def _workspace(meta, q, backward):
-    need = int(_lib().dp_xa_workspace(*meta[:6], backward))
+    need = _workspace_floats(meta, backward)
     return torch.empty(need, dtype=torch.float32, device=q.device) if need > 0 else None
 
 
@@ -83,10 +89,8 @@ def _forward(q, k, v, lens, mask, scale, need_lse):
     out = torch.empty((b, lq, hq, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((b, hk, lq * (hq // hk)), dtype=torch.float32, device=q.device) if need_lse else None
     ws = _workspace(meta, q, 0)
-    with B.on_device(q):
-        B.check(_lib().dp_xa_fwd(_p(q), _p(k), _p(v), _p(out), _p(lse), _p(lens), _p(mask),
-                                 0 if mask is None else mask.stride(0), _p(ws), _strides(q, k, v), *meta, scale,
-                                 _DTYPES[q.dtype], B.stream_ptr()), "xa_fwd")
+    B.launch("xa_fwd", _lib().dp_xa_fwd, q, _p(q), _p(k), _p(v), _p(out), _p(lse), _p(lens), _p(mask),
+             0 if mask is None else mask.stride(0), _p(ws), _strides(q, k, v), *meta, scale, _DTYPES[q.dtype])
     return out, lse
 
 
@@ -105,13 +109,12 @@ class _CrossAttention(torch.autograd.Function):
         b, lq, hq, d = q.shape
         meta = (b, lq, k.shape[1], k.shape[2], hq // k.shape[2], d)
         dout = _rows(dout)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         delta = torch.empty_like(lse)
         ws = _workspace(meta, q, 1)
-        with B.on_device(q):
-            B.check(_lib().dp_xa_bwd(_p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(delta), _p(dq), _p(dk), _p(dv),
-                                     _p(lens), _p(mask), 0 if mask is None else mask.stride(0), _p(ws),
-                                     _strides(q, k, v, dout), *meta, ctx.scale, _DTYPES[q.dtype], B.stream_ptr()), "xa_bwd")
+        B.launch("xa_bwd", _lib().dp_xa_bwd, q, _p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(delta), _p(dq), _p(dk),
+                 _p(dv), _p(lens), _p(mask), 0 if mask is None else mask.stride(0), _p(ws), _strides(q, k, v, dout), *meta,
+                 ctx.scale, _DTYPES[q.dtype])
         return dq, dk, dv, None, None, None
 
 

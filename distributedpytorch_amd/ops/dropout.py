@@ -88,10 +88,9 @@ def _run(x, residual, p, seed, use_word):
     if x.numel() == 0:
         return y
     dev = isinstance(seed, torch.Tensor)
-    with B.on_device(x):
-        B.check(_lib().dp_dropout(x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(), x.numel(),
-                                  dropout_threshold(p), 0 if dev else seed, seed.data_ptr() if dev else None,
-                                  int(use_word), _DTYPES[x.dtype], B.stream_ptr()), "dropout")
+    B.launch("dropout", _lib().dp_dropout, x, x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(),
+             x.numel(), dropout_threshold(p), 0 if dev else seed, seed.data_ptr() if dev else None, use_word,
+             _DTYPES[x.dtype])
     return y
 
 

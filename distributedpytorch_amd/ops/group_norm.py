@@ -7,6 +7,7 @@ batch, so it serves training at a few images per GPU, and evaluation computes wh
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -58,6 +59,9 @@ def group_norm_act_reference(x, num_groups, weight=None, bias=None, eps=1e-5, ac
 def _rows(t: torch.Tensor):
     """(tensor, elements between rows): ``t`` as it is when its memory is NHWC rows (a channels-last map or a channel
     slice of one), a channels-last copy otherwise."""
+    ld = t.shape[1]
+    if t.is_contiguous(memory_format=torch.channels_last):
+        return t, ld
     ld = row_stride(t)
     if ld is None:
         t = t.contiguous(memory_format=torch.channels_last)
@@ -70,17 +74,23 @@ def _p(t: Optional[torch.Tensor]):
 
 
 def _vec(t: Optional[torch.Tensor]):
-    return None if t is None else t.detach().float().contiguous()
+    if t is None:
+        return None
+    t = t.detach()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _new(x: torch.Tensor) -> torch.Tensor:
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
+    return torch.empty_like(x, memory_format=torch.channels_last)
 
 
-def _workspace(x, groups):
-    n, c, h, w = x.shape
-    return torch.empty(int(_lib().dp_gn_workspace(n, h * w, c, groups, x.element_size())), dtype=torch.float32,
-                       device=x.device)
+@functools.lru_cache(maxsize=4096)
+def _workspace_floats(n, hw, c, groups, esize) -> int:
+    return int(_lib().dp_gn_workspace(n, hw, c, groups, esize))
+
+
+def _workspace(x, n, hw, c, groups):
+    return torch.empty(_workspace_floats(n, hw, c, groups, x.element_size()), dtype=torch.float32, device=x.device)
 
 
 def _forward(x, groups, weight, bias, eps, act, residual):
@@ -92,10 +102,9 @@ def _forward(x, groups, weight, bias, eps, act, residual):
         ldr = c
         if residual is not None:
             residual, ldr = _rows(residual)
-        ws = _workspace(x, groups)
-        with B.on_device(x):
-            B.check(_lib().dp_gn_fwd(_p(x), _p(residual), _p(weight), _p(bias), _p(y), _p(stats), _p(ws), n,
-                                     h * w, c, groups, ldx, ldr, eps, act, _DTYPES[x.dtype], B.stream_ptr()), "gn_fwd")
+        ws = _workspace(x, n, h * w, c, groups)
+        B.launch("gn_fwd", _lib().dp_gn_fwd, x, _p(x), _p(residual), _p(weight), _p(bias), _p(y), _p(stats), _p(ws), n, h * w,
+                 c, groups, ldx, ldr, eps, act, _DTYPES[x.dtype])
     return y, stats
 
 
@@ -116,26 +125,28 @@ class _GroupNormAct(torch.autograd.Function):
         n, c, h, w = x.shape
         dx = _new(x)
         dres = _new(x) if residual is not None else None
-        dw = torch.empty(c, dtype=torch.float32, device=x.device) if wdtype is not None else None
-        db = torch.empty(c, dtype=torch.float32, device=x.device) if bdtype is not None else None
+        dw = None if wdtype is None else torch.empty_like(w32)
+        db = None if bdtype is None else torch.empty_like(b32)
         if x.numel():
             x, ldx = _rows(x)
             g, ldd = _rows(dy)
             ldr = c
             if residual is not None:
                 residual, ldr = _rows(residual)
-            ws = _workspace(x, groups)
-            with B.on_device(x):
-                B.check(_lib().dp_gn_bwd(_p(g), _p(x), _p(residual), _p(w32), _p(b32), _p(stats), _p(dx), _p(dres), _p(dw),
-                                         _p(db), _p(ws), n, h * w, c, groups, ldx, ldr, ldd, act,
-                                         _DTYPES[x.dtype], B.stream_ptr()), "gn_bwd")
+            ws = _workspace(x, n, h * w, c, groups)
+            B.launch("gn_bwd", _lib().dp_gn_bwd, x, _p(g), _p(x), _p(residual), _p(w32), _p(b32), _p(stats), _p(dx), _p(dres),
+                     _p(dw), _p(db), _p(ws), n, h * w, c, groups, ldx, ldr, ldd, act, _DTYPES[x.dtype])
         else:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
         if dres is None and ctx.needs_input_grad[3]:
             dres = dy                                     # no activation: the residual's gradient is dy
-        return (dx, None if dw is None else dw.to(wdtype), None if db is None else db.to(bdtype), dres, None, None, None)
+        if dw is not None and wdtype != torch.float32:
+            dw = dw.to(wdtype)
+        if db is not None and bdtype != torch.float32:
+            db = db.to(bdtype)
+        return dx, dw, db, dres, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
