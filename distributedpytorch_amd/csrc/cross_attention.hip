@@ -12,11 +12,10 @@
 // second operand of the product that contracts over them; the first operand of that product comes out of the row-major
 // LDS tile through transposing reads.
 //
-//   xa_fwd    128 rows a workgroup (32 a wave), keys in blocks of 64 through LDS, running maximum and sum; with few rows
-//             the keys are split over workgroups and xa_join puts the parts together
-//   xa_delta  delta per row
+//   xa_fwd    128 or 256 rows a workgroup (32 or 64 a wave), keys in blocks of 64 through LDS, running maximum and sum;
+//             with few rows the keys are split over workgroups and xa_join puts the parts together
+//   xa_dq     128 rows a workgroup, keys in blocks of 64; leaves delta behind for
 //   xa_dkv    128 keys a workgroup (32 a wave, their k and v in registers), rows in blocks of 32 through LDS
-//   xa_dq     128 rows a workgroup, keys in blocks of 64
 //   xa_sum    joins the fp32 parts of dq, or of dk and dv, where a long axis was split; one order, no atomics
 //
 // P and dS are rounded to the tensors' type before their second product (its operands are 16 bits wide); sums, statistics
@@ -31,14 +30,24 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 
+typedef __attribute__((ext_vector_type(2))) float f32x2v;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
 struct Bf {
     typedef bf16_raw raw;
     static __device__ __forceinline__ f32x16 mfma(const uint4& a, const uint4& b, const f32x16& c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ unsigned pair(float lo, float hi) { return pack2(lo, hi); }
+    static __device__ __forceinline__ unsigned pair(float lo, float hi) {
+        return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2v){lo, hi}, bf16x2));
+    }
     static __device__ __forceinline__ void unpair(unsigned u, float& lo, float& hi) {
         lo = __uint_as_float(u << 16); hi = __uint_as_float(u & 0xffff0000u);
+    }
+    // c + both halves of u
+    static __device__ __forceinline__ float add_pair(unsigned u, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u), (bf16x2){(__bf16)1.f, (__bf16)1.f}, c, false);
     }
 };
 
@@ -48,11 +57,13 @@ struct Hf {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ unsigned pair(float lo, float hi) {
-        const f16 a = (f16)lo, b = (f16)hi;
-        return (unsigned)__builtin_bit_cast(unsigned short, a) | ((unsigned)__builtin_bit_cast(unsigned short, b) << 16);
+        return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2v){lo, hi}, f16x2));
     }
     static __device__ __forceinline__ void unpair(unsigned u, float& lo, float& hi) {
         lo = (float)__builtin_bit_cast(f16, (unsigned short)u); hi = (float)__builtin_bit_cast(f16, (unsigned short)(u >> 16));
+    }
+    static __device__ __forceinline__ float add_pair(unsigned u, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, u), (f16x2){(f16)1.f, (f16)1.f}, c, false);
     }
 };
 
@@ -79,11 +90,23 @@ struct Att {
     float* part;                     // their fp32 partial results
 };
 
-__device__ __forceinline__ f32x16 zero16() {
+__device__ __forceinline__ f32x16 splat16(float v) {
     f32x16 z;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    for (int i = 0; i < 16; ++i) z[i] = v;
     return z;
+}
+
+__device__ __forceinline__ f32x16 zero16() { return splat16(0.f); }
+
+// the larger, or the sum, of the two lanes l and l ^ 32 (a row's two halves), on both of them
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Consecutive workgroups go round the 8 XCDs: give each XCD one contiguous range of the work, so that the workgroups
@@ -114,9 +137,13 @@ __device__ __forceinline__ int entry(int r, int h) { return 8 * (r >> 2) + 4 * h
 
 // 64-bit set of the keys of block kb that take part; every wave of the workgroup gets the same set
 __device__ __forceinline__ unsigned long long key_set(const Att& p, int b, int len, int kb) {
+    if (!p.mask) {
+        const int left = len - kb * 64;
+        return left >= 64 ? ~0ull : (1ull << left) - 1;
+    }
     const int key = kb * 64 + (int)(threadIdx.x & 63);
     bool on = key < len;
-    if (on && p.mask) on = p.mask[(long)b * p.mask_ld + key] != 0;
+    if (on) on = p.mask[(long)b * p.mask_ld + key] != 0;
     return __ballot(on);
 }
 
@@ -140,31 +167,47 @@ __device__ __forceinline__ long dense_row(const Att& p, int b, int hk, int r) {
     return (((long)b * p.Lq + l) * (p.Hk * p.share) + hk * p.share + (r - l * p.share)) * p.D;
 }
 
-// one 16-byte piece of NROWS x DP tile rows per thread and step; `ok` decides whether a row is read or zero
+// a tile of NROWS rows in LDS, moved in 16-byte pieces by the 256 threads
 template <int DP, int NROWS> struct Stage {
     static constexpr int kPieces = (NROWS * DP / 8 + 255) / 256;   // 16-byte pieces of a thread
+    static constexpr bool kWhole = NROWS * DP / 8 % 256 == 0;      // every thread has kPieces of them
     static constexpr int kLd = DP * 2 + 16;                        // LDS bytes of a row: 16 of padding spread the banks
     static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * 256) / (DP / 8); }
     static __device__ __forceinline__ int col(int i) { return ((int)threadIdx.x + i * 256) % (DP / 8) * 8; }
     static __device__ __forceinline__ void put(unsigned char* tile, const uint4 (&u)[kPieces]) {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
-            if (NROWS * DP / 8 % 256 == 0 || row(i) < NROWS) *reinterpret_cast<uint4*>(tile + row(i) * kLd + col(i) * 2) = u[i];
+            if (kWhole || row(i) < NROWS) *reinterpret_cast<uint4*>(tile + row(i) * kLd + col(i) * 2) = u[i];
     }
 };
 
-template <typename T, int DP>
-__device__ __forceinline__ void fetch_keys(const Att& p, const void* base, const View& v, int b, int hk, int kb,
-                                           unsigned long long set, uint4 (&u)[Stage<DP, kKeys>::kPieces]) {
+// the thread's pieces of successive key blocks of k or v, a block of keys ahead of their use
+template <typename T, int DP> struct KeyStream {
     typedef Stage<DP, kKeys> S;
-    const T* t = (const T*)base + b * v.b + hk * v.h;
+    const T* at[S::kPieces];
+    long step;
+    uint4 u[S::kPieces];
+    __device__ __forceinline__ void open(const void* base, const View& v, int b, int hk, int kb) {
+        const T* t = (const T*)base + b * v.b + hk * v.h;
 #pragma unroll
-    for (int i = 0; i < S::kPieces; ++i) {
-        u[i] = make_uint4(0, 0, 0, 0);
-        if (S::row(i) < kKeys && (set >> S::row(i) & 1) && S::col(i) < p.D)
-            u[i] = *reinterpret_cast<const uint4*>(t + ((long)kb * kKeys + S::row(i)) * v.l + S::col(i));
+        for (int i = 0; i < S::kPieces; ++i) at[i] = t + ((long)kb * kKeys + S::row(i)) * v.l + S::col(i);
+        step = kKeys * v.l;
     }
-}
+    __device__ __forceinline__ void next(const Att& p, unsigned long long set) {
+        if (set == ~0ull && p.D == DP && S::kWhole) {
+#pragma unroll
+            for (int i = 0; i < S::kPieces; ++i) u[i] = *reinterpret_cast<const uint4*>(at[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kPieces; ++i) {
+                u[i] = make_uint4(0, 0, 0, 0);
+                if (S::row(i) < kKeys && (set >> S::row(i) & 1) && S::col(i) < p.D) u[i] = *reinterpret_cast<const uint4*>(at[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) at[i] += step;
+    }
+};
 
 // this lane's row as the second operand (contracted over the head's width): DP / 16 pieces of 8 elements
 template <typename T, int DP>
@@ -196,54 +239,64 @@ __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename E, int DP>
-__global__ __launch_bounds__(256) void xa_fwd_kernel(Att p, int tiles) {
+// NT: row tiles of 32 of a wave.
+template <typename E, int DP, int NT>
+__global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
     typedef typename E::raw T;
     typedef Stage<DP, kKeys> S;
     __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
     __shared__ __attribute__((aligned(16))) unsigned char Vs[2][kKeys * S::kLd];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
     const Work w = work_of(p, tiles);
-    const int r = w.tile * kRows + wave * 32 + l31;
-    const bool row_on = r < p.R, wave_on = w.tile * kRows + wave * 32 < p.R;
+    const int r0 = w.tile * (kRows * NT) + wave * (32 * NT) + l31;
+    const bool wave_on = r0 - l31 < p.R;
     const int len = key_count(p, w.b);
     const int nkb = (len + kKeys - 1) / kKeys;
     const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
 
-    uint4 qf[DP / 16];
-    row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r, row_on, qf);
-    f32x16 acc[DP / 32];
+    uint4 qf[NT][DP / 16];
+    f32x16 acc[NT][DP / 32];
+    float m[NT], l[NT];
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
-    float m = -kInf, l = 0.f;
-
-    uint4 kreg[S::kPieces], vreg[S::kPieces];
+    for (int n = 0; n < NT; ++n) {
+        row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r0 + 32 * n, r0 + 32 * n < p.R, qf[n]);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) acc[n][t] = zero16();
+        m[n] = -kInf;
+        l[n] = 0.f;
+    }
+    KeyStream<T, DP> ks_, vs_;
     unsigned long long set = 0, next = 0;
     if (kb0 < kb1) {
+        ks_.open(p.k, p.vk, w.b, w.hk, kb0);
+        vs_.open(p.v, p.vv, w.b, w.hk, kb0);
         next = key_set(p, w.b, len, kb0);
-        fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb0, next, kreg);
-        fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb0, next, vreg);
+        ks_.next(p, next);
+        vs_.next(p, next);
     }
     for (int kb = kb0; kb < kb1; ++kb) {
         unsigned char *kt = Ks[kb & 1], *vt = Vs[kb & 1];
-        S::put(kt, kreg);
-        S::put(vt, vreg);
+        S::put(kt, ks_.u);
+        S::put(vt, vs_.u);
         set = next;
         __syncthreads();                     // (two buffers: the block before last is read no more)
         if (kb + 1 < kb1) {
             next = key_set(p, w.b, len, kb + 1);
-            fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb + 1, next, kreg);
-            fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb + 1, next, vreg);
+            ks_.next(p, next);
+            vs_.next(p, next);
         }
         if (!wave_on || set == 0) continue;
-        // S^T: keys on the registers, this lane's row
-        f32x16 st[2] = {zero16(), zero16()};
+        // S^T: keys on the registers, this lane's rows
+        f32x16 st[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = zero16();
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const uint4 kf = *reinterpret_cast<const uint4*>(kt + (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2);
-                st[t] = E::mfma(kf, qf[ks], st[t]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) st[n][t] = E::mfma(kf, qf[n][ks], st[n][t]);
             }
         if (set != ~0ull) {
 #pragma unroll
@@ -251,71 +304,90 @@ __global__ __launch_bounds__(256) void xa_fwd_kernel(Att p, int tiles) {
                 const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (!(bits >> entry(i, 0) & 1)) st[t][i] = -kInf;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        if (!(bits >> entry(i, 0) & 1)) st[n][t][i] = -kInf;
             }
         }
-        float mx = st[0][0];
+        uint4 pf[NT][4];
 #pragma unroll
-        for (int i = 1; i < 32; ++i) mx = fmaxf(mx, st[i >> 4][i & 15]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mnew = fmaxf(m, mx);
-        const float mc = mnew == -kInf ? 0.f : mnew * p.c;
-        if (__any(mnew != m)) {
-            const float alpha = __builtin_amdgcn_exp2f(fmaf(m, p.c, -mc));       // (m = -inf: 0)
-            l *= alpha;
+        for (int n = 0; n < NT; ++n) {
+            float mx = st[n][0][0];
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
+            for (int i = 1; i < 32; ++i) mx = __builtin_elementwise_maximum(mx, st[n][i >> 4][i & 15]);
+            mx = halves_max(mx);
+            // The reference m only follows the maximum where it is passed by more than 2^8: probabilities relative to it
+            // stay far inside both types' range, and the accumulators are seldom rescaled.
+            if (__any(!(mx * p.c <= fmaf(m[n], p.c, 8.f)))) {
+                const float top = __builtin_elementwise_maximum(m[n], mx);
+                const float alpha = top == -kInf ? 1.f : __builtin_amdgcn_exp2f((m[n] - top) * p.c);   // (m = -inf: 0)
+                l[n] *= alpha;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
-            m = mnew;
-        }
+                for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(st[t][i], p.c, -mc));
-                st[t][i] = e;
-                l += e;
+                    for (int i = 0; i < 16; ++i) acc[n][t][i] *= alpha;
+                m[n] = top;
             }
+            const float mc = m[n] == -kInf ? 0.f : m[n] * p.c;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                f32x16& x = st[n][s >> 1];
+#pragma unroll
+                for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, -mc));
+                pf[n][s] = pack_acc<E>(x, s & 1);
+                // The sum takes the rounded probabilities, two an instruction.  Over the few keys of one block their
+                // rounding would show in the sum (and in backward's probabilities): there it takes the unrounded ones.
+                if (nkb > 1)
+                    l[n] = E::add_pair(pf[n][s].w, E::add_pair(pf[n][s].z, E::add_pair(pf[n][s].y, E::add_pair(pf[n][s].x, l[n]))));
+                else
+#pragma unroll
+                    for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) l[n] += x[i];
+            }
+        }
         // O^T += V^T P^T
         const unsigned char* vb = vt + (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const uint4 pf = pack_acc<E>(st[s >> 1], s & 1);
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t) {
                 const unsigned char* a = vb + (16 * s) * S::kLd + t * 64;
-                acc[t] = E::mfma(tr_pair(a, a + 8 * S::kLd), pf, acc[t]);
+                const uint4 vf = tr_pair(a, a + 8 * S::kLd);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n][t] = E::mfma(vf, pf[n][s], acc[n][t]);
             }
-        }
     }
-    l += __shfl_xor(l, 32, 64);
-    if (!row_on) return;
     const long bh = (long)w.b * p.Hk + w.hk;
-    if (p.splits > 1) {
-        float* o = p.part + ((bh * p.splits + w.split) * p.R + r) * (DP + 2);
-        if (h == 0) { o[DP] = m; o[DP + 1] = l; }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = r0 + 32 * n;
+        const float sum = halves_sum(l[n]);
+        if (r >= p.R) continue;
+        if (p.splits > 1) {
+            float* o = p.part + ((bh * p.splits + w.split) * p.R + r) * (DP + 2);
+            if (h == 0) { o[DP] = m[n]; o[DP + 1] = sum; }
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2)
+                    *reinterpret_cast<float2*>(o + t * 32 + entry(i, h)) = make_float2(acc[n][t][i], acc[n][t][i + 1]);
+            continue;
+        }
+        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+        if (h == 0 && p.lse) p.lse[bh * p.R + r] = sum > 0.f ? fmaf(m[n], p.c, __builtin_amdgcn_logf(sum)) : kInf;
+        T* o = (T*)p.out + dense_row(p, w.b, w.hk, r);
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[t * 32 + entry(i, h)] = acc[t][i];
-        return;
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    if (h == 0 && p.lse) p.lse[bh * p.R + r] = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : kInf;
-    T* o = (T*)p.out + dense_row(p, w.b, w.hk, r);
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d = t * 32 + 8 * g + 4 * h;
-            if (d < p.D) {
-                uint2 u;
-                u.x = E::pair(acc[t][4 * g] * inv, acc[t][4 * g + 1] * inv);
-                u.y = E::pair(acc[t][4 * g + 2] * inv, acc[t][4 * g + 3] * inv);
-                *reinterpret_cast<uint2*>(o + d) = u;
+            for (int g = 0; g < 4; ++g) {
+                const int d = t * 32 + 8 * g + 4 * h;
+                if (d < p.D) {
+                    uint2 u;
+                    u.x = E::pair(acc[n][t][4 * g] * inv, acc[n][t][4 * g + 1] * inv);
+                    u.y = E::pair(acc[n][t][4 * g + 2] * inv, acc[n][t][4 * g + 3] * inv);
+                    *reinterpret_cast<uint2*>(o + d) = u;
+                }
             }
-        }
+    }
 }
 
 // joins the splits of one row: a wave per row
@@ -350,37 +422,176 @@ __global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// delta[row] = sum_d do o: 16 lanes a row
-template <typename E>
-__global__ __launch_bounds__(256) void xa_delta_kernel(Att p, long rows) {
+// dq of 128 rows, and delta for xa_dkv.  delta = rowsum(do o) comes from the rounded o; over a few keys o is as large as
+// v and that rounding would show in dS = P (dP - delta), so an image whose keys fit one block takes
+// delta = sum_j P_j dP_j from its registers instead.
+template <typename E, int DP>
+__global__ __launch_bounds__(256, 2) void xa_dq_kernel(Att p, int tiles) {
     typedef typename E::raw T;
-    const long id = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int g = threadIdx.x & 15;
-    if (id >= rows) return;
-    const long bh = id / p.R;
-    const int r = (int)(id - bh * p.R);
-    const int b = (int)(bh / p.Hk), hk = (int)(bh % p.Hk);
-    const T* o = (const T*)p.o + dense_row(p, b, hk, r);
-    const T* d = (const T*)p.dout + row_at(p, p.vd, b, hk, r);
-    float s = 0.f;
-    if (g * 8 < p.D) {
-        const uint4 a = *reinterpret_cast<const uint4*>(o + g * 8), c = *reinterpret_cast<const uint4*>(d + g * 8);
-        const unsigned av[4] = {a.x, a.y, a.z, a.w}, cv[4] = {c.x, c.y, c.z, c.w};
+    typedef Stage<DP, kKeys> S;
+    __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
+    __shared__ __attribute__((aligned(16))) unsigned char Vs[2][kKeys * S::kLd];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+    const Work w = work_of(p, tiles);
+    const int r = w.tile * kRows + wave * 32 + l31;
+    const bool row_on = r < p.R, wave_on = w.tile * kRows + wave * 32 < p.R;
+    const int len = key_count(p, w.b);
+    const int nkb = (len + kKeys - 1) / kKeys;
+    const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
+    const long bh = (long)w.b * p.Hk + w.hk;
+
+    uint4 qf[DP / 16], df[DP / 16];
+    row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r, row_on, qf);
+    row_operand<T, DP>(p, p.dout, p.vd, w.b, w.hk, r, row_on, df);
+    const float lse = row_on ? p.lse[bh * p.R + r] : kInf;
+    float del = 0.f;
+    if (nkb > 1) {
+        uint4 of[DP / 16];
+        const View vo = {(long)p.R * p.Hk * p.D, (long)p.share * p.Hk * p.D, p.D};
+        row_operand<T, DP>(p, p.o, vo, w.b, w.hk, r, row_on, of);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float a0, a1, c0, c1;
-            E::unpair(av[i], a0, a1);
-            E::unpair(cv[i], c0, c1);
-            s = fmaf(a0, c0, fmaf(a1, c1, s));
+        for (int ks = 0; ks < DP / 16; ++ks) {
+            const unsigned a[4] = {of[ks].x, of[ks].y, of[ks].z, of[ks].w}, c[4] = {df[ks].x, df[ks].y, df[ks].z, df[ks].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float a0, a1, c0, c1;
+                E::unpair(a[i], a0, a1);
+                E::unpair(c[i], c0, c1);
+                del = fmaf(a0, c0, fmaf(a1, c1, del));
+            }
+        }
+        del = halves_sum(del);
+        if (w.split == 0 && row_on && h == 0) p.delta[bh * p.R + r] = del;
+    }
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
+
+    KeyStream<T, DP> ks_, vs_;
+    unsigned long long set = 0, next = 0;
+    if (kb0 < kb1) {
+        ks_.open(p.k, p.vk, w.b, w.hk, kb0);
+        vs_.open(p.v, p.vv, w.b, w.hk, kb0);
+        next = key_set(p, w.b, len, kb0);
+        ks_.next(p, next);
+        vs_.next(p, next);
+    }
+    for (int kb = kb0; kb < kb1; ++kb) {
+        unsigned char *kt = Ks[kb & 1], *vt = Vs[kb & 1];
+        S::put(kt, ks_.u);
+        S::put(vt, vs_.u);
+        set = next;
+        __syncthreads();
+        if (kb + 1 < kb1) {
+            next = key_set(p, w.b, len, kb + 1);
+            ks_.next(p, next);
+            vs_.next(p, next);
+        }
+        if (!wave_on || set == 0) continue;
+        // P and dP - delta of 32 keys: keys on the registers, this lane's row
+        auto scores = [&](int t, f32x16& s, f32x16& dp) {
+            s = zero16();
+            dp = splat16(-del);
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                const int at = (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
+                s = E::mfma(*reinterpret_cast<const uint4*>(kt + at), qf[ks], s);
+                dp = E::mfma(*reinterpret_cast<const uint4*>(vt + at), df[ks], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse));
+            if (set != ~0ull) {
+                const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = (bits >> entry(i, 0) & 1) ? s[i] : 0.f;
+            }
+        };
+        if (nkb == 1) {
+            float sum = 0.f;
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                f32x16 s, dp;
+                scores(t, s, dp);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum = fmaf(s[i], dp[i], sum);
+            }
+            del = halves_sum(sum);
+            if (row_on && h == 0) p.delta[bh * p.R + r] = del;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 s, dp;
+            scores(t, s, dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= dp[i];
+            const unsigned char* kb_ = kt + (t * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd +
+                                       (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint4 sf = pack_acc<E>(s, k);
+#pragma unroll
+                for (int u = 0; u < DP / 32; ++u) {
+                    const unsigned char* a = kb_ + (16 * k) * S::kLd + u * 64;
+                    acc[u] = E::mfma(tr_pair(a, a + 8 * S::kLd), sf, acc[u]);
+                }
+            }
         }
     }
+    if (!row_on) return;
+    const long at = dense_row(p, w.b, w.hk, r);
+    const long whole = (long)p.B * p.Hk * p.R * p.D;
 #pragma unroll
-    for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
-    if (g == 0) p.delta[id] = s;
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = t * 32 + 8 * g + 4 * h;
+            if (d >= p.D) continue;
+            if (p.splits > 1) {
+                *reinterpret_cast<float4*>(p.part + (long)w.split * whole + at + d) =
+                    make_float4(acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]);
+            } else {
+                uint2 u;
+                u.x = E::pair(acc[t][4 * g] * p.scale, acc[t][4 * g + 1] * p.scale);
+                u.y = E::pair(acc[t][4 * g + 2] * p.scale, acc[t][4 * g + 3] * p.scale);
+                *reinterpret_cast<uint2*>((T*)p.dq + at + d) = u;
+            }
+        }
 }
 
+// the thread's pieces of successive row blocks of q or dout
+template <typename T, int DP> struct RowStream {
+    typedef Stage<DP, kStep> S;
+    const T* base;
+    const T* at[S::kPieces];
+    uint4 u[S::kPieces];
+    __device__ __forceinline__ void open(const Att& p, const void* t, const View& v, int b, int hk, int st) {
+        base = (const T*)t;
+#pragma unroll
+        for (int i = 0; i < S::kPieces; ++i) at[i] = base + row_at(p, v, b, hk, st * kStep + S::row(i)) + S::col(i);
+    }
+    __device__ __forceinline__ void next(const Att& p, const View& v, int b, int hk, int st) {
+        if (st * kStep + kStep <= p.R && p.D == DP && S::kWhole) {
+#pragma unroll
+            for (int i = 0; i < S::kPieces; ++i) u[i] = *reinterpret_cast<const uint4*>(at[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kPieces; ++i) {
+                u[i] = make_uint4(0, 0, 0, 0);
+                if (S::row(i) < kStep && st * kStep + S::row(i) < p.R && S::col(i) < p.D) u[i] = *reinterpret_cast<const uint4*>(at[i]);
+            }
+        }
+        if (kStep % p.share == 0) {
+            const long step = kStep / p.share * v.l;
+#pragma unroll
+            for (int i = 0; i < S::kPieces; ++i) at[i] += step;
+        } else {
+            open(p, base, v, b, hk, st + 1);
+        }
+    }
+};
+
 template <typename E, int DP>
-__global__ __launch_bounds__(256) void xa_dkv_kernel(Att p, int tiles) {
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, int tiles) {
     typedef typename E::raw T;
     typedef Stage<DP, kStep> S;
     __shared__ __attribute__((aligned(16))) unsigned char Qs[2][kStep * S::kLd];
@@ -392,7 +603,7 @@ __global__ __launch_bounds__(256) void xa_dkv_kernel(Att p, int tiles) {
     const int len = key_count(p, w.b);
     bool on = key < len;
     if (on && p.mask) on = p.mask[(long)w.b * p.mask_ld + key] != 0;
-    const bool wave_on = __any(on);
+    const bool wave_on = __any(on), wave_all = __all(on);
     const long bh = (long)w.b * p.Hk + w.hk;
     const int nst = (p.R + kStep - 1) / kStep;
     const int st0 = (int)((long)nst * w.split / p.splits);
@@ -412,54 +623,58 @@ __global__ __launch_bounds__(256) void xa_dkv_kernel(Att p, int tiles) {
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
 
-    uint4 qreg[S::kPieces], dreg[S::kPieces];
+    RowStream<T, DP> qs, ds;
+    const bool first = threadIdx.x < kStep, second = threadIdx.x >= kStep && threadIdx.x < 2 * kStep;
+    const float* lp = (first ? p.lse : p.delta) + bh * p.R;
     float lreg = 0.f;
     auto fetch = [&](int st) {
-#pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) {
-            const int r = st * kStep + S::row(i);
-            qreg[i] = dreg[i] = make_uint4(0, 0, 0, 0);
-            if (S::row(i) < kStep && r < p.R && S::col(i) < p.D) {
-                qreg[i] = *reinterpret_cast<const uint4*>((const T*)p.q + row_at(p, p.vq, w.b, w.hk, r) + S::col(i));
-                dreg[i] = *reinterpret_cast<const uint4*>((const T*)p.dout + row_at(p, p.vd, w.b, w.hk, r) + S::col(i));
-            }
-        }
-        if (threadIdx.x < 2 * kStep) {                       // a row beyond the last: P = 2^(0 - inf) = 0, delta = 0
+        qs.next(p, p.vq, w.b, w.hk, st);
+        ds.next(p, p.vd, w.b, w.hk, st);
+        if (first || second) {                               // a row beyond the last: P = 2^(0 - inf) = 0, delta = 0
             const int r = st * kStep + (int)(threadIdx.x & (kStep - 1));
-            lreg = threadIdx.x < kStep ? kInf : 0.f;
-            if (r < p.R) lreg = (threadIdx.x < kStep ? p.lse : p.delta)[bh * p.R + r];
+            lreg = first ? kInf : 0.f;
+            if (r < p.R) lreg = first ? lp[r] : -lp[r];
         }
     };
-    if (st0 < st1) fetch(st0);
+    if (st0 < st1) {
+        qs.open(p, p.q, p.vq, w.b, w.hk, st0);
+        ds.open(p, p.dout, p.vd, w.b, w.hk, st0);
+        fetch(st0);
+    }
     for (int st = st0; st < st1; ++st) {
         const int buf = st & 1;
         unsigned char *qt = Qs[buf], *dt = Ds[buf];
-        S::put(qt, qreg);
-        S::put(dt, dreg);
-        if (threadIdx.x < 2 * kStep) Ls[buf][threadIdx.x / kStep][threadIdx.x & (kStep - 1)] = lreg;
+        S::put(qt, qs.u);
+        S::put(dt, ds.u);
+        if (first || second) Ls[buf][second][threadIdx.x & (kStep - 1)] = lreg;
         __syncthreads();
         if (st + 1 < st1) fetch(st + 1);
         if (!wave_on) continue;
-        // S and dP: rows on the registers, this lane's key
-        f32x16 s = zero16(), dp = zero16();
+        // S and dP - delta: rows on the registers, this lane's key
+        f32x16 s = zero16(), dp;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][1][8 * g + 4 * h]);
+            dp[4 * g] = x.x; dp[4 * g + 1] = x.y; dp[4 * g + 2] = x.z; dp[4 * g + 3] = x.w;
+        }
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
             const int at = l31 * S::kLd + (ks * 16 + h * 8) * 2;
             s = E::mfma(*reinterpret_cast<const uint4*>(qt + at), kf[ks], s);
             dp = E::mfma(*reinterpret_cast<const uint4*>(dt + at), vf[ks], dp);
         }
-        float lse[16], del[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            *reinterpret_cast<float4*>(lse + 4 * g) = *reinterpret_cast<const float4*>(&Ls[buf][0][8 * g + 4 * h]);
-            *reinterpret_cast<float4*>(del + 4 * g) = *reinterpret_cast<const float4*>(&Ls[buf][1][8 * g + 4 * h]);
-        }
+            const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][0][8 * g + 4 * h]);
+            const float lse[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float e = on ? __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse[i])) : 0.f;
-            s[i] = e;
-            dp[i] = e * (dp[i] - del[i]);
+            for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + i], p.c, -lse[i]));
         }
+        if (!wave_all)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = on ? s[i] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] *= s[i];
         const int tr = (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -497,98 +712,6 @@ __global__ __launch_bounds__(256) void xa_dkv_kernel(Att p, int tiles) {
         }
 }
 
-template <typename E, int DP>
-__global__ __launch_bounds__(256) void xa_dq_kernel(Att p, int tiles) {
-    typedef typename E::raw T;
-    typedef Stage<DP, kKeys> S;
-    __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
-    __shared__ __attribute__((aligned(16))) unsigned char Vs[2][kKeys * S::kLd];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
-    const Work w = work_of(p, tiles);
-    const int r = w.tile * kRows + wave * 32 + l31;
-    const bool row_on = r < p.R, wave_on = w.tile * kRows + wave * 32 < p.R;
-    const int len = key_count(p, w.b);
-    const int nkb = (len + kKeys - 1) / kKeys;
-    const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
-    const long bh = (long)w.b * p.Hk + w.hk;
-
-    uint4 qf[DP / 16], df[DP / 16];
-    row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r, row_on, qf);
-    row_operand<T, DP>(p, p.dout, p.vd, w.b, w.hk, r, row_on, df);
-    const float lse = row_on ? p.lse[bh * p.R + r] : kInf, del = row_on ? p.delta[bh * p.R + r] : 0.f;
-    f32x16 acc[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
-
-    uint4 kreg[S::kPieces], vreg[S::kPieces];
-    unsigned long long set = 0, next = 0;
-    if (kb0 < kb1) {
-        next = key_set(p, w.b, len, kb0);
-        fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb0, next, kreg);
-        fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb0, next, vreg);
-    }
-    for (int kb = kb0; kb < kb1; ++kb) {
-        unsigned char *kt = Ks[kb & 1], *vt = Vs[kb & 1];
-        S::put(kt, kreg);
-        S::put(vt, vreg);
-        set = next;
-        __syncthreads();
-        if (kb + 1 < kb1) {
-            next = key_set(p, w.b, len, kb + 1);
-            fetch_keys<T, DP>(p, p.k, p.vk, w.b, w.hk, kb + 1, next, kreg);
-            fetch_keys<T, DP>(p, p.v, p.vv, w.b, w.hk, kb + 1, next, vreg);
-        }
-        if (!wave_on || set == 0) continue;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                const int at = (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
-                s = E::mfma(*reinterpret_cast<const uint4*>(kt + at), qf[ks], s);
-                dp = E::mfma(*reinterpret_cast<const uint4*>(vt + at), df[ks], dp);
-            }
-            const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float e = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse));
-                if (set != ~0ull) e = (bits >> entry(i, 0) & 1) ? e : 0.f;
-                s[i] = e * (dp[i] - del);
-            }
-            const unsigned char* kb_ = kt + (t * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd +
-                                       (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint4 sf = pack_acc<E>(s, k);
-#pragma unroll
-                for (int u = 0; u < DP / 32; ++u) {
-                    const unsigned char* a = kb_ + (16 * k) * S::kLd + u * 64;
-                    acc[u] = E::mfma(tr_pair(a, a + 8 * S::kLd), sf, acc[u]);
-                }
-            }
-        }
-    }
-    if (!row_on) return;
-    const long at = dense_row(p, w.b, w.hk, r);
-    const long whole = (long)p.B * p.Hk * p.R * p.D;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d = t * 32 + 8 * g + 4 * h;
-            if (d >= p.D) continue;
-            if (p.splits > 1) {
-                *reinterpret_cast<float4*>(p.part + (long)w.split * whole + at + d) =
-                    make_float4(acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]);
-            } else {
-                uint2 u;
-                u.x = E::pair(acc[t][4 * g] * p.scale, acc[t][4 * g + 1] * p.scale);
-                u.y = E::pair(acc[t][4 * g + 2] * p.scale, acc[t][4 * g + 3] * p.scale);
-                *reinterpret_cast<uint2*>((T*)p.dq + at + d) = u;
-            }
-        }
-}
-
 // out[i] = factor * sum over parts of part[s][i], four elements a thread
 template <typename E>
 __global__ __launch_bounds__(256) void xa_sum_kernel(const float* part, long stride, int parts, long count, float factor,
@@ -608,25 +731,38 @@ __global__ __launch_bounds__(256) void xa_sum_kernel(const float* part, long str
 
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 
-// parts of a long axis of `steps` blocks: enough for about two workgroups a CU, at least four blocks a part
-int parts_for(long groups, long steps) {
-    long n = (512 + groups - 1) / groups;
-    const long most = (steps + 3) / 4;
-    if (n > most) n = most;
-    return (int)(n < 1 ? 1 : n);
+// Parts of a long axis: `groups` workgroups of `steps` blocks each run in rounds of `slots` workgroups, so the time goes
+// with rounds / parts; each part more costs the join about `extra` blocks' time, and none is shorter than four blocks.
+int parts_for(long groups, long steps, long slots, double extra) {
+    const long most = (steps + 3) / 4 < 64 ? (steps + 3) / 4 : 64;
+    int best = 1;
+    double least = 1e300;
+    for (long n = 1; n <= most; ++n) {
+        const double rounds = (double)((groups * n + slots - 1) / slots);
+        const double cost = rounds * (double)((steps + n - 1) / n) + (n > 1 ? extra * (double)n * (double)groups / slots : 0.0);
+        if (cost < least * 0.98) { least = cost; best = (int)n; }
+    }
+    return best;
 }
 
-struct Plan { long fwd_groups, dkv_groups; int rtiles, ktiles, fwd, dkv, dq, dp; };
+constexpr long kCus = 256;
+
+struct Plan { long fwd_groups, dq_groups, dkv_groups; int fwd_tiles, dq_tiles, ktiles, nt, fwd, dkv, dq, dp; };
 
 Plan plan_of(int B, long R, int Lk, int Hk, int D) {
     Plan n;
     n.dp = padded(D);
-    n.rtiles = (int)((R + kRows - 1) / kRows);
+    n.nt = n.dp <= 64 && R > kRows ? 2 : 1;
+    n.fwd_tiles = (int)((R + kRows * n.nt - 1) / (kRows * n.nt));
+    n.dq_tiles = (int)((R + kRows - 1) / kRows);
     n.ktiles = (Lk + kRows - 1) / kRows;
-    n.fwd_groups = (long)B * Hk * n.rtiles;
+    n.fwd_groups = (long)B * Hk * n.fwd_tiles;
+    n.dq_groups = (long)B * Hk * n.dq_tiles;
     n.dkv_groups = (long)B * Hk * n.ktiles;
-    n.fwd = n.dq = parts_for(n.fwd_groups, (Lk + kKeys - 1) / kKeys);
-    n.dkv = parts_for(n.dkv_groups, (R + kStep - 1) / kStep);
+    const long keys = (Lk + kKeys - 1) / kKeys;
+    n.fwd = parts_for(n.fwd_groups, keys, 2 * kCus, 1.0);
+    n.dq = parts_for(n.dq_groups, keys, 2 * kCus, 1.0);
+    n.dkv = parts_for(n.dkv_groups, (R + kStep - 1) / kStep, (n.dp <= 64 ? 2 : 1) * kCus, 4.0);
     return n;
 }
 
@@ -641,18 +777,24 @@ template <typename E, int DP> int launch_fwd(Att p, const Plan& n, hipStream_t s
     p.splits = n.fwd;
     const long blocks = n.fwd_groups * n.fwd, rows = (long)p.B * p.Hk * p.R;
     if (bad_grid(blocks) || bad_grid((rows + 3) / 4)) return -3;
-    xa_fwd_kernel<E, DP><<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.rtiles);
+    if constexpr (DP <= 64) {
+        if (n.nt == 2) xa_fwd_kernel<E, DP, 2><<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
+    }
+    if (n.nt == 1) xa_fwd_kernel<E, DP, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
     if (n.fwd > 1) xa_join_kernel<E, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, rows);
     return DP_LAUNCH_STATUS();
 }
 
 template <typename E, int DP> int launch_bwd(Att p, const Plan& n, hipStream_t st) {
     typedef typename E::raw T;
-    const long rows = (long)p.B * p.Hk * p.R, kv = (long)p.B * p.Lk * p.Hk * p.D, qn = rows * p.D;
-    if (bad_grid((rows + 15) / 16) || bad_grid(n.dkv_groups * n.dkv) || bad_grid(n.fwd_groups * n.dq) ||
-        bad_grid((kv + 1023) / 1024) || bad_grid((qn + 1023) / 1024))
+    const long kv = (long)p.B * p.Lk * p.Hk * p.D, qn = (long)p.B * p.Hk * p.R * p.D;
+    if (bad_grid(n.dkv_groups * n.dkv) || bad_grid(n.dq_groups * n.dq) || bad_grid((kv + 1023) / 1024) ||
+        bad_grid((qn + 1023) / 1024))
         return -3;
-    xa_delta_kernel<E><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, st>>>(p, rows);
+    p.splits = n.dq;
+    xa_dq_kernel<E, DP><<<dim3((unsigned)(n.dq_groups * n.dq)), 256, 0, st>>>(p, n.dq_tiles);
+    if (n.dq > 1)
+        xa_sum_kernel<E><<<dim3((unsigned)((qn + 1023) / 1024)), 256, 0, st>>>(p.part, qn, n.dq, qn, p.scale, (T*)p.dq);
     p.splits = n.dkv;
     xa_dkv_kernel<E, DP><<<dim3((unsigned)(n.dkv_groups * n.dkv)), 256, 0, st>>>(p, n.ktiles);
     if (n.dkv > 1) {
@@ -660,10 +802,6 @@ template <typename E, int DP> int launch_bwd(Att p, const Plan& n, hipStream_t s
         xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part, 2 * kv, n.dkv, kv, p.scale, (T*)p.dk);
         xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part + kv, 2 * kv, n.dkv, kv, 1.f, (T*)p.dv);
     }
-    p.splits = n.dq;
-    xa_dq_kernel<E, DP><<<dim3((unsigned)(n.fwd_groups * n.dq)), 256, 0, st>>>(p, n.rtiles);
-    if (n.dq > 1)
-        xa_sum_kernel<E><<<dim3((unsigned)((qn + 1023) / 1024)), 256, 0, st>>>(p.part, qn, n.dq, qn, p.scale, (T*)p.dq);
     return DP_LAUNCH_STATUS();
 }
 
