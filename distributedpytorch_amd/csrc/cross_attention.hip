@@ -135,6 +135,13 @@ template <typename E> __device__ __forceinline__ uint4 pack_acc(const f32x16& a,
 // entry of the 32 that accumulator register r of lane half h belongs to
 __device__ __forceinline__ int entry(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
+__device__ __forceinline__ float row_max(const f32x16 (&s)[2]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = __builtin_elementwise_maximum(mx, s[i >> 4][i & 15]);
+    return mx;
+}
+
 // 64-bit set of the keys of block kb that take part; every wave of the workgroup gets the same set
 __device__ __forceinline__ unsigned long long key_set(const Att& p, int b, int len, int kb) {
     if (!p.mask) {
@@ -223,6 +230,10 @@ __device__ __forceinline__ void row_operand(const Att& p, const void* base, cons
     }
 }
 
+// In the kernels below no branch stands between a matrix instruction and the first use of its result by an ordinary one:
+// where a branch joined again before that use, the compiler counted the wait of the longer way only, and on the shorter
+// one the registers were read before they were written.  So results are used first and masks are put in afterwards.
+
 struct Work { int b, hk, tile, split; };
 
 // work item: tiles fastest, then splits, then (image, key head)
@@ -298,6 +309,9 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) st[n][t] = E::mfma(kf, qf[n][ks], st[n][t]);
             }
+        float top[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) top[n] = row_max(st[n]);
         if (set != ~0ull) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -305,28 +319,26 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        if (!(bits >> entry(i, 0) & 1)) st[n][t][i] = -kInf;
+                    for (int n = 0; n < NT; ++n) st[n][t][i] = (bits >> entry(i, 0) & 1) ? st[n][t][i] : -kInf;
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) top[n] = row_max(st[n]);
         }
         uint4 pf[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float mx = st[n][0][0];
-#pragma unroll
-            for (int i = 1; i < 32; ++i) mx = __builtin_elementwise_maximum(mx, st[n][i >> 4][i & 15]);
-            mx = halves_max(mx);
+            const float mx = halves_max(top[n]);
             // The reference m only follows the maximum where it is passed by more than 2^8: probabilities relative to it
             // stay far inside both types' range, and the accumulators are seldom rescaled.
             if (__any(!(mx * p.c <= fmaf(m[n], p.c, 8.f)))) {
-                const float top = __builtin_elementwise_maximum(m[n], mx);
-                const float alpha = top == -kInf ? 1.f : __builtin_amdgcn_exp2f((m[n] - top) * p.c);   // (m = -inf: 0)
+                const float up = __builtin_elementwise_maximum(m[n], mx);
+                const float alpha = up == -kInf ? 1.f : __builtin_amdgcn_exp2f((m[n] - up) * p.c);   // (m = -inf: 0)
                 l[n] *= alpha;
 #pragma unroll
                 for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[n][t][i] *= alpha;
-                m[n] = top;
+                m[n] = up;
             }
             const float mc = m[n] == -kInf ? 0.f : m[n] * p.c;
 #pragma unroll
@@ -335,9 +347,9 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
 #pragma unroll
                 for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, -mc));
                 pf[n][s] = pack_acc<E>(x, s & 1);
-                // The sum takes the rounded probabilities, two an instruction.  Over the few keys of one block their
-                // rounding would show in the sum (and in backward's probabilities): there it takes the unrounded ones.
-                if (nkb > 1)
+                // The sum takes the rounded probabilities, two an instruction.  Over few keys their rounding would show
+                // in the sum (and in backward's probabilities): there it takes the unrounded ones.
+                if (nkb > 4)
                     l[n] = E::add_pair(pf[n][s].w, E::add_pair(pf[n][s].z, E::add_pair(pf[n][s].y, E::add_pair(pf[n][s].x, l[n]))));
                 else
 #pragma unroll
@@ -426,7 +438,7 @@ __global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
 // v and that rounding would show in dS = P (dP - delta), so an image whose keys fit one block takes
 // delta = sum_j P_j dP_j from its registers instead.
 template <typename E, int DP>
-__global__ __launch_bounds__(256, 2) void xa_dq_kernel(Att p, int tiles) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int tiles) {
     typedef typename E::raw T;
     typedef Stage<DP, kKeys> S;
     __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
@@ -488,10 +500,10 @@ __global__ __launch_bounds__(256, 2) void xa_dq_kernel(Att p, int tiles) {
             vs_.next(p, next);
         }
         if (!wave_on || set == 0) continue;
-        // P and dP - delta of 32 keys: keys on the registers, this lane's row
-        auto scores = [&](int t, f32x16& s, f32x16& dp) {
+        // P (dP - delta) of 32 keys: keys on the registers, this lane's row
+        auto scores = [&](int t, f32x16& s) {
             s = zero16();
-            dp = splat16(-del);
+            f32x16 dp = splat16(-del);
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) {
                 const int at = (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
@@ -499,7 +511,7 @@ __global__ __launch_bounds__(256, 2) void xa_dq_kernel(Att p, int tiles) {
                 dp = E::mfma(*reinterpret_cast<const uint4*>(vt + at), df[ks], dp);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse));
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse)) * dp[i];
             if (set != ~0ull) {
                 const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
 #pragma unroll
@@ -510,20 +522,19 @@ __global__ __launch_bounds__(256, 2) void xa_dq_kernel(Att p, int tiles) {
             float sum = 0.f;
 #pragma unroll 1
             for (int t = 0; t < 2; ++t) {
-                f32x16 s, dp;
-                scores(t, s, dp);
+                f32x16 s;
+                scores(t, s);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum = fmaf(s[i], dp[i], sum);
+                for (int i = 0; i < 16; ++i) sum += s[i];
             }
             del = halves_sum(sum);
             if (row_on && h == 0) p.delta[bh * p.R + r] = del;
+            if (__popcll(set) == 1) continue;             // a single key: P = 1 whatever the score, dq = dk = 0
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            f32x16 s, dp;
-            scores(t, s, dp);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] *= dp[i];
+            f32x16 s;
+            scores(t, s);
             const unsigned char* kb_ = kt + (t * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd +
                                        (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
@@ -590,6 +601,8 @@ template <typename T, int DP> struct RowStream {
     }
 };
 
+// dk and dv of 128 keys.  A key is a column of every product here, so what a masked key's lane computes reaches no other:
+// it is thrown away at the end.
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, int tiles) {
     typedef typename E::raw T;
@@ -603,7 +616,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
     const int len = key_count(p, w.b);
     bool on = key < len;
     if (on && p.mask) on = p.mask[(long)w.b * p.mask_ld + key] != 0;
-    const bool wave_on = __any(on), wave_all = __all(on);
+    const bool wave_on = __any(on);
     const long bh = (long)w.b * p.Hk + w.hk;
     const int nst = (p.R + kStep - 1) / kStep;
     const int st0 = (int)((long)nst * w.split / p.splits);
@@ -670,9 +683,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + i], p.c, -lse[i]));
         }
-        if (!wave_all)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = on ? s[i] : 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] *= s[i];
         const int tr = (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
@@ -688,6 +698,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
         }
     }
     if (key >= p.Lk) return;
+    const bool lone = len <= 64 && __popcll(key_set(p, w.b, len, 0)) == 1;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) {
+        if (!on) dv[t] = zero16();
+        if (!on || lone) dk[t] = zero16();
+    }
     const long at = (((long)w.b * p.Lk + key) * p.Hk + w.hk) * p.D;
     const long whole = (long)p.B * p.Lk * p.Hk * p.D;
 #pragma unroll
@@ -761,7 +777,7 @@ Plan plan_of(int B, long R, int Lk, int Hk, int D) {
     n.dkv_groups = (long)B * Hk * n.ktiles;
     const long keys = (Lk + kKeys - 1) / kKeys;
     n.fwd = parts_for(n.fwd_groups, keys, 2 * kCus, 1.0);
-    n.dq = parts_for(n.dq_groups, keys, 2 * kCus, 1.0);
+    n.dq = parts_for(n.dq_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, 1.0);
     n.dkv = parts_for(n.dkv_groups, (R + kStep - 1) / kStep, (n.dp <= 64 ? 2 : 1) * kCus, 4.0);
     return n;
 }

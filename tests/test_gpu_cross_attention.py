@@ -234,6 +234,22 @@ def test_cross_attention_replays(shape):
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
 
 
+@pytest.mark.parametrize("kind", ["one key", "length", "mask"])
+def test_cross_attention_over_a_single_key_has_no_score_gradient(kind):
+    """P = 1 whatever the score: dq and dk are zeros, not roundings of them."""
+    from distributedpytorch_amd import ops
+    q, k, v, dout = _inputs(2, 50, 1 if kind == "one key" else 60, 4, 2, 64, torch.bfloat16, 13)
+    lens = torch.tensor([1, 1], dtype=torch.int32, device="cuda") if kind == "length" else None
+    mask = None
+    if kind == "mask":
+        mask = torch.zeros(2, 60, dtype=torch.bool, device="cuda")
+        mask[0, 7] = mask[1, 59] = True
+    _check(q, k, v, dout, lens, mask)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(ops.cross_attention(*leaves, key_lengths=lens, key_mask=mask), leaves, dout)
+    assert not dq.any() and not dk.any() and dv.any()
+
+
 def test_cross_attention_without_a_graph_equals_with_one():
     from distributedpytorch_amd import ops
     q, k, v, _ = _inputs(2, 70, 90, 2, 2, 64, torch.float16, 12)
