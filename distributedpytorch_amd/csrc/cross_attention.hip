@@ -15,7 +15,7 @@
 //   xa_fwd    128 or 256 rows a workgroup (32 or 64 a wave), keys in blocks of 64 through LDS, running maximum and sum;
 //             with few rows the keys are split over workgroups and xa_join puts the parts together
 //   xa_dq     128 rows a workgroup, keys in blocks of 64; leaves delta behind for
-//   xa_dkv    128 keys a workgroup (32 a wave, their k and v in registers), rows in blocks of 32 through LDS
+//   xa_dkv    128 keys a workgroup (32 a wave, their k and v in registers), rows in blocks of 64 through LDS
 //   xa_sum    joins the fp32 parts of dq, or of dk and dv, where a long axis was split; one order, no atomics
 //
 // P and dS are rounded to the tensors' type before their second product (its operands are 16 bits wide); sums, statistics
@@ -69,7 +69,7 @@ struct Hf {
 
 constexpr int kRows = 128;       // rows (forward, dq) or keys (dkv) of a workgroup: 4 waves x 32
 constexpr int kKeys = 64;        // keys of an LDS block (forward, dq)
-constexpr int kStep = 32;        // rows of an LDS block (dkv)
+constexpr int kStep = 64;        // rows of an LDS block (dkv)
 constexpr float kInf = __builtin_huge_valf();
 
 // strides in elements: image, position, head (elements of a head are adjacent)
@@ -663,37 +663,40 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
         __syncthreads();
         if (st + 1 < st1) fetch(st + 1);
         if (!wave_on) continue;
-        // S and dP - delta: rows on the registers, this lane's key
-        f32x16 s = zero16(), dp;
+        // 32 rows at a time: S and dP - delta with rows on the registers, this lane's key
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][1][8 * g + 4 * h]);
-            dp[4 * g] = x.x; dp[4 * g + 1] = x.y; dp[4 * g + 2] = x.z; dp[4 * g + 3] = x.w;
-        }
+        for (int sub = 0; sub < kStep / 32; ++sub) {
+            f32x16 s = zero16(), dp;
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-            const int at = l31 * S::kLd + (ks * 16 + h * 8) * 2;
-            s = E::mfma(*reinterpret_cast<const uint4*>(qt + at), kf[ks], s);
-            dp = E::mfma(*reinterpret_cast<const uint4*>(dt + at), vf[ks], dp);
-        }
+            for (int g = 0; g < 4; ++g) {
+                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][1][sub * 32 + 8 * g + 4 * h]);
+                dp[4 * g] = x.x; dp[4 * g + 1] = x.y; dp[4 * g + 2] = x.z; dp[4 * g + 3] = x.w;
+            }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][0][8 * g + 4 * h]);
-            const float lse[4] = {x.x, x.y, x.z, x.w};
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                const int at = (sub * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
+                s = E::mfma(*reinterpret_cast<const uint4*>(qt + at), kf[ks], s);
+                dp = E::mfma(*reinterpret_cast<const uint4*>(dt + at), vf[ks], dp);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + i], p.c, -lse[i]));
-        }
+            for (int g = 0; g < 4; ++g) {
+                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][0][sub * 32 + 8 * g + 4 * h]);
+                const float lse[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dp[i] *= s[i];
-        const int tr = (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+                for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + i], p.c, -lse[i]));
+            }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint4 pf = pack_acc<E>(s, k), df = pack_acc<E>(dp, k);
+            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
+            const int tr = (sub * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t) {
-                const int at = tr + (16 * k) * S::kLd + t * 64;
-                dv[t] = E::mfma(tr_pair(dt + at, dt + at + 8 * S::kLd), pf, dv[t]);
-                dk[t] = E::mfma(tr_pair(qt + at, qt + at + 8 * S::kLd), df, dk[t]);
+            for (int k = 0; k < 2; ++k) {
+                const uint4 pf = pack_acc<E>(s, k), df = pack_acc<E>(dp, k);
+#pragma unroll
+                for (int t = 0; t < DP / 32; ++t) {
+                    const int at = tr + (16 * k) * S::kLd + t * 64;
+                    dv[t] = E::mfma(tr_pair(dt + at, dt + at + 8 * S::kLd), pf, dv[t]);
+                    dk[t] = E::mfma(tr_pair(qt + at, qt + at + 8 * S::kLd), df, dk[t]);
+                }
             }
         }
     }
