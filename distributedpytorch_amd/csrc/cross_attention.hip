@@ -646,7 +646,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
         if (first || second) {                               // a row beyond the last: P = 2^(0 - inf) = 0, delta = 0
             const int r = st * kStep + (int)(threadIdx.x & (kStep - 1));
             lreg = first ? kInf : 0.f;
-            if (r < p.R) lreg = first ? lp[r] : -lp[r];
+            if (r < p.R) lreg = lp[r];                       // (its use, and its wait, come with the next block)
         }
     };
     if (st0 < st1) {
@@ -659,46 +659,59 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
         unsigned char *qt = Qs[buf], *dt = Ds[buf];
         S::put(qt, qs.u);
         S::put(dt, ds.u);
-        if (first || second) Ls[buf][second][threadIdx.x & (kStep - 1)] = lreg;
+        if (first || second) Ls[buf][second][threadIdx.x & (kStep - 1)] = second ? -lreg : lreg;
         __syncthreads();
         if (st + 1 < st1) fetch(st + 1);
         if (!wave_on) continue;
-        // 32 rows at a time: S and dP - delta with rows on the registers, this lane's key
-#pragma unroll
-        for (int sub = 0; sub < kStep / 32; ++sub) {
-            f32x16 s = zero16(), dp;
+        // Two halves of 32 rows, the vector work of each beside the matrix work of the other: products(1) with
+        // probabilities(0), then gradients(0) with probabilities(1).
+        f32x16 s[2], dp[2];
+        uint4 pf[2][2], df[2][2];
+        auto products = [&](int u) {                      // S and dP - delta: rows on the registers, this lane's key
+            s[u] = zero16();
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][1][sub * 32 + 8 * g + 4 * h]);
-                dp[4 * g] = x.x; dp[4 * g + 1] = x.y; dp[4 * g + 2] = x.z; dp[4 * g + 3] = x.w;
+                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][1][u * 32 + 8 * g + 4 * h]);
+                dp[u][4 * g] = x.x; dp[u][4 * g + 1] = x.y; dp[u][4 * g + 2] = x.z; dp[u][4 * g + 3] = x.w;
             }
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) {
-                const int at = (sub * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
-                s = E::mfma(*reinterpret_cast<const uint4*>(qt + at), kf[ks], s);
-                dp = E::mfma(*reinterpret_cast<const uint4*>(dt + at), vf[ks], dp);
+                const int at = (u * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
+                s[u] = E::mfma(*reinterpret_cast<const uint4*>(qt + at), kf[ks], s[u]);
+                dp[u] = E::mfma(*reinterpret_cast<const uint4*>(dt + at), vf[ks], dp[u]);
             }
+        };
+        auto probabilities = [&](int u) {                 // P and dS, packed
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][0][sub * 32 + 8 * g + 4 * h]);
+                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][0][u * 32 + 8 * g + 4 * h]);
                 const float lse[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + i], p.c, -lse[i]));
+                for (int i = 0; i < 4; ++i) {
+                    s[u][4 * g + i] = __builtin_amdgcn_exp2f(fmaf(s[u][4 * g + i], p.c, -lse[i]));
+                    dp[u][4 * g + i] *= s[u][4 * g + i];
+                }
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] *= s[i];
-            const int tr = (sub * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+            for (int k = 0; k < 2; ++k) { pf[u][k] = pack_acc<E>(s[u], k); df[u][k] = pack_acc<E>(dp[u], k); }
+        };
+        auto gradients = [&](int u) {
+            const int tr = (u * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint4 pf = pack_acc<E>(s, k), df = pack_acc<E>(dp, k);
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int t = 0; t < DP / 32; ++t) {
                     const int at = tr + (16 * k) * S::kLd + t * 64;
-                    dv[t] = E::mfma(tr_pair(dt + at, dt + at + 8 * S::kLd), pf, dv[t]);
-                    dk[t] = E::mfma(tr_pair(qt + at, qt + at + 8 * S::kLd), df, dk[t]);
+                    dv[t] = E::mfma(tr_pair(dt + at, dt + at + 8 * S::kLd), pf[u][k], dv[t]);
+                    dk[t] = E::mfma(tr_pair(qt + at, qt + at + 8 * S::kLd), df[u][k], dk[t]);
                 }
-            }
-        }
+        };
+        products(0);
+        probabilities(0);
+        gradients(0);
+        products(1);
+        probabilities(1);
+        gradients(1);
     }
     if (key >= p.Lk) return;
     const bool lone = len <= 64 && __popcll(key_set(p, w.b, len, 0)) == 1;
