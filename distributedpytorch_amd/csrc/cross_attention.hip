@@ -252,7 +252,7 @@ __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
 // ------------------------------------------------------------------------------------------------ forward
 // NT: row tiles of 32 of a wave.
 template <typename E, int DP, int NT>
-__global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
+__global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 3 : 2) void xa_fwd_kernel(Att p, int tiles) {
     typedef typename E::raw T;
     typedef Stage<DP, kKeys> S;
     __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
@@ -297,8 +297,22 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
             vs_.next(p, next);
         }
         if (!wave_on || set == 0) continue;
-        // S^T: keys on the registers, this lane's rows
         f32x16 st[NT][2];
+        float top[NT], mc[NT];
+        uint4 pf[NT][4];
+        auto probabilities = [&](int n) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                f32x16& x = st[n][s >> 1];
+#pragma unroll
+                for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) {
+                    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, -mc[n]));
+                    l[n] += x[i];
+                }
+                pf[n][s] = pack_acc<E>(x, s & 1);
+            }
+        };
+        // S^T: keys on the registers, this lane's rows
 #pragma unroll
         for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = zero16();
 #pragma unroll
@@ -309,7 +323,6 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) st[n][t] = E::mfma(kf, qf[n][ks], st[n][t]);
             }
-        float top[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) top[n] = row_max(st[n]);
         if (set != ~0ull) {
@@ -324,14 +337,18 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) top[n] = row_max(st[n]);
         }
-        uint4 pf[NT][4];
+        bool rises = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float mx = halves_max(top[n]);
-            // The reference m only follows the maximum where it is passed by more than 2^8: probabilities relative to it
-            // stay far inside both types' range, and the accumulators are seldom rescaled.
-            if (__any(!(mx * p.c <= fmaf(m[n], p.c, 8.f)))) {
-                const float up = __builtin_elementwise_maximum(m[n], mx);
+            top[n] = halves_max(top[n]);
+            rises |= !(top[n] * p.c <= fmaf(m[n], p.c, 8.f));
+        }
+        // The reference m only follows the maximum where it is passed by more than 2^8: probabilities relative to it stay
+        // far inside both types' range, and the accumulators are seldom rescaled.
+        if (__any(rises)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float up = __builtin_elementwise_maximum(m[n], top[n]);
                 const float alpha = up == -kInf ? 1.f : __builtin_amdgcn_exp2f((m[n] - up) * p.c);   // (m = -inf: 0)
                 l[n] *= alpha;
 #pragma unroll
@@ -340,22 +357,11 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(Att p, int tiles) {
                     for (int i = 0; i < 16; ++i) acc[n][t][i] *= alpha;
                 m[n] = up;
             }
-            const float mc = m[n] == -kInf ? 0.f : m[n] * p.c;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                f32x16& x = st[n][s >> 1];
-#pragma unroll
-                for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, -mc));
-                pf[n][s] = pack_acc<E>(x, s & 1);
-                // The sum takes the rounded probabilities, two an instruction.  Over few keys their rounding would show
-                // in the sum (and in backward's probabilities): there it takes the unrounded ones.
-                if (nkb > 4)
-                    l[n] = E::add_pair(pf[n][s].w, E::add_pair(pf[n][s].z, E::add_pair(pf[n][s].y, E::add_pair(pf[n][s].x, l[n]))));
-                else
-#pragma unroll
-                    for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) l[n] += x[i];
-            }
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mc[n] = m[n] == -kInf ? 0.f : m[n] * p.c;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) probabilities(n);
         // O^T += V^T P^T
         const unsigned char* vb = vt + (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
@@ -784,7 +790,7 @@ struct Plan { long fwd_groups, dq_groups, dkv_groups; int fwd_tiles, dq_tiles, k
 Plan plan_of(int B, long R, int Lk, int Hk, int D) {
     Plan n;
     n.dp = padded(D);
-    n.nt = n.dp <= 64 && R > kRows ? 2 : 1;
+    n.nt = n.dp < 64 && R > kRows ? 2 : 1;
     n.fwd_tiles = (int)((R + kRows * n.nt - 1) / (kRows * n.nt));
     n.dq_tiles = (int)((R + kRows - 1) / kRows);
     n.ktiles = (Lk + kRows - 1) / kRows;
