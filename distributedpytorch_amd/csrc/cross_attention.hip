@@ -78,7 +78,7 @@ struct View { long b, l, h; };
 struct Att {
     const void *q, *k, *v, *o, *dout;
     void *out, *dq, *dk, *dv;
-    float *lse, *delta;              // [B, Hk, R]: log2 of the row's sum of exponentials (+inf: no key), rowsum(do o)
+    float *lse, *delta;              // [B, Hk, R]: log2 of the row's sum of exponentials (+inf: no key), -rowsum(do o)
     const int* lens;                 // [B] keys of each image, or null
     const unsigned char* mask;       // [B, Lk], nonzero = takes part, or null
     long mask_ld;
@@ -174,45 +174,135 @@ __device__ __forceinline__ long dense_row(const Att& p, int b, int hk, int r) {
     return (((long)b * p.Lq + l) * (p.Hk * p.share) + hk * p.share + (r - l * p.share)) * p.D;
 }
 
-// a tile of NROWS rows in LDS, moved in 16-byte pieces by the 256 threads
-template <int DP, int NROWS> struct Stage {
-    static constexpr int kPieces = (NROWS * DP / 8 + 255) / 256;   // 16-byte pieces of a thread
-    static constexpr bool kWhole = NROWS * DP / 8 % 256 == 0;      // every thread has kPieces of them
-    static constexpr int kLd = DP * 2 + 16;                        // LDS bytes of a row: 16 of padding spread the banks
-    static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * 256) / (DP / 8); }
-    static __device__ __forceinline__ int col(int i) { return ((int)threadIdx.x + i * 256) % (DP / 8) * 8; }
-    static __device__ __forceinline__ void put(unsigned char* tile, const uint4 (&u)[kPieces]) {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-            if (kWhole || row(i) < NROWS) *reinterpret_cast<uint4*>(tile + row(i) * kLd + col(i) * 2) = u[i];
+// A tile of 64 rows in LDS.  A row's 16-byte chunks lie permuted (chunk c of row r in slot c ^ swz(r)): rows that share
+// banks then keep the same chunk in different ones, for whole-row reads (32 rows, one chunk) and for transposing reads
+// (4 rows, 4 chunks) alike.  Piece j of a thread has the place (wave kPieces + j) 1024 + 16 lane, as LDS-DMA writes it: the
+// permutation is made by what the lane reads.
+template <int DP> struct Tile {
+    static constexpr int kPitch = DP == 96 ? 256 : DP * 2;         // bytes of a row: a power of two
+    static constexpr int kBytes = 64 * kPitch;
+    static constexpr int kPieces = kBytes / 4096;                  // of each of 256 threads
+    static __device__ __forceinline__ int swz(int r) {
+        return DP == 32 ? (r >> 2) & 3 : DP == 64 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3);
+    }
+    static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+    static __device__ __forceinline__ int place(int j) { return (wave() * kPieces + j) * 1024 + ((int)threadIdx.x & 63) * 16; }
+    static __device__ __forceinline__ int row(int j) { return place(j) / kPitch; }
+    static __device__ __forceinline__ int col(int j) { return ((place(j) % kPitch / 16) ^ swz(row(j))) * 8; }    // element
+};
+
+// Where this lane reads a tile: whole rows (32 of them, 8 elements a lane) and their transposes.
+template <int DP> struct Reads {
+    int row, tr;
+    __device__ __forceinline__ Reads() {
+        typedef Tile<DP> L;
+        const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5, q = (lane & 15) >> 2;
+        row = l31 * L::kPitch + ((h ^ L::swz(l31)) << 4);
+        tr = (4 * h + q) * L::kPitch + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ L::swz(4 * h + q)) << 4) + (lane & 1) * 8;
+    }
+    // elements 16 ks + 8 h .. of row 32 t + lane
+    __device__ __forceinline__ uint4 rows(const unsigned char* tile, int t, int ks) const {
+        return *reinterpret_cast<const uint4*>(tile + t * 32 * Tile<DP>::kPitch + (row ^ (ks << 5)));
+    }
+    // column 32 t + lane of rows 16 s + 4 h + {0..3} and 16 s + 8 + 4 h + {0..3}
+    __device__ __forceinline__ uint4 cols(const unsigned char* tile, int s, int t) const {
+        const unsigned char* a = tile + 16 * s * Tile<DP>::kPitch;
+        return tr_pair(a + (tr ^ (t << 6)), a + 8 * Tile<DP>::kPitch + (tr ^ (t << 6) ^ 32));
     }
 };
 
-// the thread's pieces of successive key blocks of k or v, a block of keys ahead of their use
-template <typename T, int DP> struct KeyStream {
-    typedef Stage<DP, kKeys> S;
-    const T* at[S::kPieces];
-    long step;
-    uint4 u[S::kPieces];
-    __device__ __forceinline__ void open(const void* base, const View& v, int b, int hk, int kb) {
-        const T* t = (const T*)base + b * v.b + hk * v.h;
+constexpr unsigned kOut = 0x80000000u;       // an offset that every buffer descriptor below answers with zeros
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* base, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+
+__device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t from, unsigned char* to, unsigned offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
+}
+
+// Successive tiles of rows, brought a tile ahead of their use.  DMA: straight into LDS, rows and columns that do not exist
+// as zeros; otherwise (masked keys, whose rows must become zeros whatever they hold; strides or head shares that do not
+// fit 32-bit offsets from a tile's first row) through registers.
+template <typename T, int DP, bool DMA> struct Stream {
+    typedef Tile<DP> L;
+    unsigned off[DMA ? L::kPieces : 1];
+    uint4 u[DMA ? 1 : L::kPieces];
+    // byte offset of piece j's row from the tile's first: a multiple of it for keys, position and head for rows
+    __device__ __forceinline__ void open(int D, long ld, long head, int share) {
+        if constexpr (DMA) {
 #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) at[i] = t + ((long)kb * kKeys + S::row(i)) * v.l + S::col(i);
-        step = kKeys * v.l;
-    }
-    __device__ __forceinline__ void next(const Att& p, unsigned long long set) {
-        if (set == ~0ull && p.D == DP && S::kWhole) {
-#pragma unroll
-            for (int i = 0; i < S::kPieces; ++i) u[i] = *reinterpret_cast<const uint4*>(at[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::kPieces; ++i) {
-                u[i] = make_uint4(0, 0, 0, 0);
-                if (S::row(i) < kKeys && (set >> S::row(i) & 1) && S::col(i) < p.D) u[i] = *reinterpret_cast<const uint4*>(at[i]);
+            for (int j = 0; j < L::kPieces; ++j) {
+                const int r = L::row(j);
+                off[j] = L::col(j) < D ? (unsigned)((r / share * ld + r % share * head + L::col(j)) * 2) : kOut;
             }
         }
+    }
+    __device__ __forceinline__ void load(const T* tile, unsigned char* to, int rows) {
+        const __amdgpu_buffer_rsrc_t from = buffer_at(tile, 0x7fffffffu);
+        if (rows >= 64) {
 #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) at[i] += step;
+            for (int j = 0; j < L::kPieces; ++j) dma(from, to + (L::wave() * L::kPieces + j) * 1024, off[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < L::kPieces; ++j)
+                dma(from, to + (L::wave() * L::kPieces + j) * 1024, L::row(j) < rows ? off[j] : kOut);
+        }
+    }
+    __device__ __forceinline__ void put(unsigned char* to) const {
+#pragma unroll
+        for (int j = 0; j < L::kPieces; ++j) *reinterpret_cast<uint4*>(to + L::place(j)) = u[j];
+    }
+};
+
+template <typename T, int DP, bool DMA> struct KeyStream : Stream<T, DP, DMA> {
+    typedef Tile<DP> L;
+    const T* base;
+    long ld;
+    __device__ __forceinline__ KeyStream(const Att& p, const void* t, const View& v, int b, int hk) {
+        base = (const T*)t + b * v.b + hk * v.h;
+        ld = v.l;
+        this->open(p.D, ld, 0, 1);
+    }
+    __device__ __forceinline__ void fetch(const Att& p, unsigned char* to, int kb, int len, unsigned long long set) {
+        const T* tile = base + (long)kb * kKeys * ld;
+        if constexpr (DMA) {
+            this->load(tile, to, len - kb * kKeys);
+        } else {
+#pragma unroll
+            for (int j = 0; j < L::kPieces; ++j) {
+                this->u[j] = make_uint4(0, 0, 0, 0);
+                if ((set >> L::row(j) & 1) && L::col(j) < p.D)
+                    this->u[j] = *reinterpret_cast<const uint4*>(tile + L::row(j) * ld + L::col(j));
+            }
+        }
+    }
+};
+
+template <typename T, int DP, bool DMA> struct RowStream : Stream<T, DP, DMA> {
+    typedef Tile<DP> L;
+    const T* base;
+    long step;                               // elements between the first rows of successive tiles (DMA: 64 % share == 0)
+    __device__ __forceinline__ RowStream(const Att& p, const void* t, const View& v, int b, int hk) {
+        base = (const T*)t;
+        step = 0;
+        if constexpr (DMA) {
+            base += b * v.b + (long)hk * p.share * v.h;
+            step = kStep / p.share * v.l;
+        }
+        this->open(p.D, v.l, v.h, p.share);
+    }
+    __device__ __forceinline__ void fetch(const Att& p, const View& v, int b, int hk, unsigned char* to, int st) {
+        if constexpr (DMA) {
+            this->load(base + st * step, to, p.R - st * kStep);
+        } else {
+#pragma unroll
+            for (int j = 0; j < L::kPieces; ++j) {
+                const int r = st * kStep + L::row(j);
+                this->u[j] = make_uint4(0, 0, 0, 0);
+                if (r < p.R && L::col(j) < p.D) this->u[j] = *reinterpret_cast<const uint4*>(base + row_at(p, v, b, hk, r) + L::col(j));
+            }
+        }
     }
 };
 
@@ -234,6 +324,12 @@ __device__ __forceinline__ void row_operand(const Att& p, const void* base, cons
 // where a branch joined again before that use, the compiler counted the wait of the longer way only, and on the shorter
 // one the registers were read before they were written.  So results are used first and masks are put in afterwards.
 
+// Every wave's DMA has landed and every wave's reads of the other buffer are done.
+__device__ __forceinline__ void arrive() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 struct Work { int b, hk, tile, split; };
 
 // work item: tiles fastest, then splits, then (image, key head)
@@ -251,12 +347,12 @@ __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
 
 // ------------------------------------------------------------------------------------------------ forward
 // NT: row tiles of 32 of a wave.
-template <typename E, int DP, int NT>
-__global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 3 : 2) void xa_fwd_kernel(Att p, int tiles) {
+template <typename E, int DP, int NT, bool DMA>
+__global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, int tiles) {
     typedef typename E::raw T;
-    typedef Stage<DP, kKeys> S;
-    __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
-    __shared__ __attribute__((aligned(16))) unsigned char Vs[2][kKeys * S::kLd];
+    // (four variables, not an array: the compiler then knows that what is brought into one is not what is read)
+    __shared__ __attribute__((aligned(16))) unsigned char K0[Tile<DP>::kBytes], V0[Tile<DP>::kBytes], K1[Tile<DP>::kBytes],
+        V1[Tile<DP>::kBytes];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
     const Work w = work_of(p, tiles);
     const int r0 = w.tile * (kRows * NT) + wave * (32 * NT) + l31;
@@ -276,27 +372,28 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 3 : 2) void xa_fwd_kerne
         m[n] = -kInf;
         l[n] = 0.f;
     }
-    KeyStream<T, DP> ks_, vs_;
+    const Reads<DP> rd;
+    KeyStream<T, DP, DMA> ks_(p, p.k, p.vk, w.b, w.hk), vs_(p, p.v, p.vv, w.b, w.hk);
     unsigned long long set = 0, next = 0;
     if (kb0 < kb1) {
-        ks_.open(p.k, p.vk, w.b, w.hk, kb0);
-        vs_.open(p.v, p.vv, w.b, w.hk, kb0);
         next = key_set(p, w.b, len, kb0);
-        ks_.next(p, next);
-        vs_.next(p, next);
+        ks_.fetch(p, K0, kb0, len, next);
+        vs_.fetch(p, V0, kb0, len, next);
     }
-    for (int kb = kb0; kb < kb1; ++kb) {
-        unsigned char *kt = Ks[kb & 1], *vt = Vs[kb & 1];
-        S::put(kt, ks_.u);
-        S::put(vt, vs_.u);
+    // one block of keys from (kt, vt), the next on its way into (kn, vn)
+    auto block = [&](unsigned char* kt, unsigned char* vt, unsigned char* kn, unsigned char* vn, int kb) {
+        if constexpr (!DMA) {
+            ks_.put(kt);
+            vs_.put(vt);
+        }
         set = next;
-        __syncthreads();                     // (two buffers: the block before last is read no more)
+        arrive();                            // this block has landed; nobody reads (kn, vn) any more
         if (kb + 1 < kb1) {
             next = key_set(p, w.b, len, kb + 1);
-            ks_.next(p, next);
-            vs_.next(p, next);
+            ks_.fetch(p, kn, kb + 1, len, next);
+            vs_.fetch(p, vn, kb + 1, len, next);
         }
-        if (!wave_on || set == 0) continue;
+        if (!wave_on || set == 0) return;
         f32x16 st[NT][2];
         float top[NT], mc[NT];
         uint4 pf[NT][4];
@@ -319,7 +416,7 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 3 : 2) void xa_fwd_kerne
         for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint4 kf = *reinterpret_cast<const uint4*>(kt + (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2);
+                const uint4 kf = rd.rows(kt, t, ks);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) st[n][t] = E::mfma(kf, qf[n][ks], st[n][t]);
             }
@@ -363,16 +460,18 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 3 : 2) void xa_fwd_kerne
 #pragma unroll
         for (int n = 0; n < NT; ++n) probabilities(n);
         // O^T += V^T P^T
-        const unsigned char* vb = vt + (4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t) {
-                const unsigned char* a = vb + (16 * s) * S::kLd + t * 64;
-                const uint4 vf = tr_pair(a, a + 8 * S::kLd);
+                const uint4 vf = rd.cols(vt, s, t);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) acc[n][t] = E::mfma(vf, pf[n][s], acc[n][t]);
             }
+    };
+    for (int kb = kb0; kb < kb1; kb += 2) {
+        block(K0, V0, K1, V1, kb);
+        if (kb + 1 < kb1) block(K1, V1, K0, V0, kb + 1);
     }
     const long bh = (long)w.b * p.Hk + w.hk;
 #pragma unroll
@@ -443,12 +542,11 @@ __global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
 // dq of 128 rows, and delta for xa_dkv.  delta = rowsum(do o) comes from the rounded o; over a few keys o is as large as
 // v and that rounding would show in dS = P (dP - delta), so an image whose keys fit one block takes
 // delta = sum_j P_j dP_j from its registers instead.
-template <typename E, int DP>
+template <typename E, int DP, bool DMA>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int tiles) {
     typedef typename E::raw T;
-    typedef Stage<DP, kKeys> S;
-    __shared__ __attribute__((aligned(16))) unsigned char Ks[2][kKeys * S::kLd];
-    __shared__ __attribute__((aligned(16))) unsigned char Vs[2][kKeys * S::kLd];
+    __shared__ __attribute__((aligned(16))) unsigned char K0[Tile<DP>::kBytes], V0[Tile<DP>::kBytes], K1[Tile<DP>::kBytes],
+        V1[Tile<DP>::kBytes];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
     const Work w = work_of(p, tiles);
     const int r = w.tile * kRows + wave * 32 + l31;
@@ -479,42 +577,41 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
             }
         }
         del = halves_sum(del);
-        if (w.split == 0 && row_on && h == 0) p.delta[bh * p.R + r] = del;
+        if (w.split == 0 && row_on && h == 0) p.delta[bh * p.R + r] = -del;
     }
     f32x16 acc[DP / 32];
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
 
-    KeyStream<T, DP> ks_, vs_;
+    const Reads<DP> rd;
+    KeyStream<T, DP, DMA> ks_(p, p.k, p.vk, w.b, w.hk), vs_(p, p.v, p.vv, w.b, w.hk);
     unsigned long long set = 0, next = 0;
     if (kb0 < kb1) {
-        ks_.open(p.k, p.vk, w.b, w.hk, kb0);
-        vs_.open(p.v, p.vv, w.b, w.hk, kb0);
         next = key_set(p, w.b, len, kb0);
-        ks_.next(p, next);
-        vs_.next(p, next);
+        ks_.fetch(p, K0, kb0, len, next);
+        vs_.fetch(p, V0, kb0, len, next);
     }
-    for (int kb = kb0; kb < kb1; ++kb) {
-        unsigned char *kt = Ks[kb & 1], *vt = Vs[kb & 1];
-        S::put(kt, ks_.u);
-        S::put(vt, vs_.u);
+    auto block = [&](unsigned char* kt, unsigned char* vt, unsigned char* kn, unsigned char* vn, int kb) {
+        if constexpr (!DMA) {
+            ks_.put(kt);
+            vs_.put(vt);
+        }
         set = next;
-        __syncthreads();
+        arrive();
         if (kb + 1 < kb1) {
             next = key_set(p, w.b, len, kb + 1);
-            ks_.next(p, next);
-            vs_.next(p, next);
+            ks_.fetch(p, kn, kb + 1, len, next);
+            vs_.fetch(p, vn, kb + 1, len, next);
         }
-        if (!wave_on || set == 0) continue;
+        if (!wave_on || set == 0) return;
         // P (dP - delta) of 32 keys: keys on the registers, this lane's row
         auto scores = [&](int t, f32x16& s) {
             s = zero16();
             f32x16 dp = splat16(-del);
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) {
-                const int at = (t * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
-                s = E::mfma(*reinterpret_cast<const uint4*>(kt + at), qf[ks], s);
-                dp = E::mfma(*reinterpret_cast<const uint4*>(vt + at), df[ks], dp);
+                s = E::mfma(rd.rows(kt, t, ks), qf[ks], s);
+                dp = E::mfma(rd.rows(vt, t, ks), df[ks], dp);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse)) * dp[i];
@@ -534,25 +631,24 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
                 for (int i = 0; i < 16; ++i) sum += s[i];
             }
             del = halves_sum(sum);
-            if (row_on && h == 0) p.delta[bh * p.R + r] = del;
-            if (__popcll(set) == 1) continue;             // a single key: P = 1 whatever the score, dq = dk = 0
+            if (row_on && h == 0) p.delta[bh * p.R + r] = -del;
+            if (__popcll(set) == 1) return;             // a single key: P = 1 whatever the score, dq = dk = 0
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 s;
             scores(t, s);
-            const unsigned char* kb_ = kt + (t * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd +
-                                       (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const uint4 sf = pack_acc<E>(s, k);
 #pragma unroll
-                for (int u = 0; u < DP / 32; ++u) {
-                    const unsigned char* a = kb_ + (16 * k) * S::kLd + u * 64;
-                    acc[u] = E::mfma(tr_pair(a, a + 8 * S::kLd), sf, acc[u]);
-                }
+                for (int u = 0; u < DP / 32; ++u) acc[u] = E::mfma(rd.cols(kt, 2 * t + k, u), sf, acc[u]);
             }
         }
+    };
+    for (int kb = kb0; kb < kb1; kb += 2) {
+        block(K0, V0, K1, V1, kb);
+        if (kb + 1 < kb1) block(K1, V1, K0, V0, kb + 1);
     }
     if (!row_on) return;
     const long at = dense_row(p, w.b, w.hk, r);
@@ -575,47 +671,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
         }
 }
 
-// the thread's pieces of successive row blocks of q or dout
-template <typename T, int DP> struct RowStream {
-    typedef Stage<DP, kStep> S;
-    const T* base;
-    const T* at[S::kPieces];
-    uint4 u[S::kPieces];
-    __device__ __forceinline__ void open(const Att& p, const void* t, const View& v, int b, int hk, int st) {
-        base = (const T*)t;
-#pragma unroll
-        for (int i = 0; i < S::kPieces; ++i) at[i] = base + row_at(p, v, b, hk, st * kStep + S::row(i)) + S::col(i);
-    }
-    __device__ __forceinline__ void next(const Att& p, const View& v, int b, int hk, int st) {
-        if (st * kStep + kStep <= p.R && p.D == DP && S::kWhole) {
-#pragma unroll
-            for (int i = 0; i < S::kPieces; ++i) u[i] = *reinterpret_cast<const uint4*>(at[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::kPieces; ++i) {
-                u[i] = make_uint4(0, 0, 0, 0);
-                if (S::row(i) < kStep && st * kStep + S::row(i) < p.R && S::col(i) < p.D) u[i] = *reinterpret_cast<const uint4*>(at[i]);
-            }
-        }
-        if (kStep % p.share == 0) {
-            const long step = kStep / p.share * v.l;
-#pragma unroll
-            for (int i = 0; i < S::kPieces; ++i) at[i] += step;
-        } else {
-            open(p, base, v, b, hk, st + 1);
-        }
-    }
-};
-
 // dk and dv of 128 keys.  A key is a column of every product here, so what a masked key's lane computes reaches no other:
 // it is thrown away at the end.
-template <typename E, int DP>
+template <typename E, int DP, bool DMA>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, int tiles) {
     typedef typename E::raw T;
-    typedef Stage<DP, kStep> S;
-    __shared__ __attribute__((aligned(16))) unsigned char Qs[2][kStep * S::kLd];
-    __shared__ __attribute__((aligned(16))) unsigned char Ds[2][kStep * S::kLd];
-    __shared__ __attribute__((aligned(16))) float Ls[2][2][kStep];
+    __shared__ __attribute__((aligned(16))) unsigned char Q0[Tile<DP>::kBytes], D0[Tile<DP>::kBytes], Q1[Tile<DP>::kBytes],
+        D1[Tile<DP>::kBytes];
+    __shared__ __attribute__((aligned(16))) float S0[2][kStep], S1[2][kStep];        // log of the sum | -delta of the rows
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
     const Work w = work_of(p, tiles);
     const int key = w.tile * kRows + wave * 32 + l31;
@@ -642,55 +705,48 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
 
-    RowStream<T, DP> qs, ds;
-    const bool first = threadIdx.x < kStep, second = threadIdx.x >= kStep && threadIdx.x < 2 * kStep;
-    const float* lp = (first ? p.lse : p.delta) + bh * p.R;
-    float lreg = 0.f;
-    auto fetch = [&](int st) {
-        qs.next(p, p.vq, w.b, w.hk, st);
-        ds.next(p, p.vd, w.b, w.hk, st);
-        if (first || second) {                               // a row beyond the last: P = 2^(0 - inf) = 0, delta = 0
-            const int r = st * kStep + (int)(threadIdx.x & (kStep - 1));
-            lreg = first ? kInf : 0.f;
-            if (r < p.R) lreg = lp[r];                       // (its use, and its wait, come with the next block)
-        }
+    const Reads<DP> rd;
+    RowStream<T, DP, DMA> qs(p, p.q, p.vq, w.b, w.hk), ds(p, p.dout, p.vd, w.b, w.hk);
+    // Rows beyond the last are zeros everywhere, statistics included: P = 1 there meets zeros of q and dout.
+    const __amdgpu_buffer_rsrc_t lse = buffer_at(p.lse + bh * p.R, p.R * 4u), del = buffer_at(p.delta + bh * p.R, p.R * 4u);
+    auto fetch = [&](unsigned char* qn, unsigned char* dn, float (*sn)[kStep], int st) {
+        qs.fetch(p, p.vq, w.b, w.hk, qn, st);
+        ds.fetch(p, p.vd, w.b, w.hk, dn, st);
+        const int wv = Tile<DP>::wave();
+        if (wv < 2)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wv ? del : lse, (__attribute__((address_space(3))) void*)sn[wv], 4,
+                                                     (unsigned)(st * kStep + lane) * 4u, 0, 0, 0);
     };
-    if (st0 < st1) {
-        qs.open(p, p.q, p.vq, w.b, w.hk, st0);
-        ds.open(p, p.dout, p.vd, w.b, w.hk, st0);
-        fetch(st0);
-    }
-    for (int st = st0; st < st1; ++st) {
-        const int buf = st & 1;
-        unsigned char *qt = Qs[buf], *dt = Ds[buf];
-        S::put(qt, qs.u);
-        S::put(dt, ds.u);
-        if (first || second) Ls[buf][second][threadIdx.x & (kStep - 1)] = second ? -lreg : lreg;
-        __syncthreads();
-        if (st + 1 < st1) fetch(st + 1);
-        if (!wave_on) continue;
-        // Two halves of 32 rows, the vector work of each beside the matrix work of the other: products(1) with
-        // probabilities(0), then gradients(0) with probabilities(1).
+    if (st0 < st1) fetch(Q0, D0, S0, st0);
+    auto block = [&](unsigned char* qt, unsigned char* dt, float (*sv)[kStep], unsigned char* qn, unsigned char* dn,
+                     float (*sn)[kStep], int st) {
+        if constexpr (!DMA) {
+            qs.put(qt);
+            ds.put(dt);
+        }
+        arrive();
+        if (st + 1 < st1) fetch(qn, dn, sn, st + 1);
+        if (!wave_on) return;
+        // two halves of 32 rows
         f32x16 s[2], dp[2];
         uint4 pf[2][2], df[2][2];
         auto products = [&](int u) {                      // S and dP - delta: rows on the registers, this lane's key
             s[u] = zero16();
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][1][u * 32 + 8 * g + 4 * h]);
+                const float4 x = *reinterpret_cast<const float4*>(&sv[1][u * 32 + 8 * g + 4 * h]);
                 dp[u][4 * g] = x.x; dp[u][4 * g + 1] = x.y; dp[u][4 * g + 2] = x.z; dp[u][4 * g + 3] = x.w;
             }
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) {
-                const int at = (u * 32 + l31) * S::kLd + (ks * 16 + h * 8) * 2;
-                s[u] = E::mfma(*reinterpret_cast<const uint4*>(qt + at), kf[ks], s[u]);
-                dp[u] = E::mfma(*reinterpret_cast<const uint4*>(dt + at), vf[ks], dp[u]);
+                s[u] = E::mfma(rd.rows(qt, u, ks), kf[ks], s[u]);
+                dp[u] = E::mfma(rd.rows(dt, u, ks), vf[ks], dp[u]);
             }
         };
         auto probabilities = [&](int u) {                 // P and dS, packed
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4 x = *reinterpret_cast<const float4*>(&Ls[buf][0][u * 32 + 8 * g + 4 * h]);
+                const float4 x = *reinterpret_cast<const float4*>(&sv[0][u * 32 + 8 * g + 4 * h]);
                 const float lse[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -702,14 +758,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
             for (int k = 0; k < 2; ++k) { pf[u][k] = pack_acc<E>(s[u], k); df[u][k] = pack_acc<E>(dp[u], k); }
         };
         auto gradients = [&](int u) {
-            const int tr = (u * 32 + 4 * h + ((lane & 15) >> 2)) * S::kLd + (((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int t = 0; t < DP / 32; ++t) {
-                    const int at = tr + (16 * k) * S::kLd + t * 64;
-                    dv[t] = E::mfma(tr_pair(dt + at, dt + at + 8 * S::kLd), pf[u][k], dv[t]);
-                    dk[t] = E::mfma(tr_pair(qt + at, qt + at + 8 * S::kLd), df[u][k], dk[t]);
+                    dv[t] = E::mfma(rd.cols(dt, 2 * u + k, t), pf[u][k], dv[t]);
+                    dk[t] = E::mfma(rd.cols(qt, 2 * u + k, t), df[u][k], dk[t]);
                 }
         };
         products(0);
@@ -718,6 +772,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
         products(1);
         probabilities(1);
         gradients(1);
+    };
+    for (int st = st0; st < st1; st += 2) {
+        block(Q0, D0, S0, Q1, D1, S1, st);
+        if (st + 1 < st1) block(Q1, D1, S1, Q0, D0, S0, st + 1);
     }
     if (key >= p.Lk) return;
     const bool lone = len <= 64 && __popcll(key_set(p, w.b, len, 0)) == 1;
@@ -806,19 +864,32 @@ Plan plan_of(int B, long R, int Lk, int Hk, int D) {
 
 bool bad(int B, int Lq, int Lk, int Hk, int share, int D) {
     return B <= 0 || Lq <= 0 || Lk <= 0 || Hk <= 0 || share <= 0 || D <= 0 || D % 8 || D > 128 ||
-           (long)Lq * share > 0x7fffff00L || (long)B * Hk * share > 0x7fffffffL || Lk > 0x7fffff00;
+           (long)Lq * share > (1L << 29) || (long)B * Hk * share > 0x7fffffffL || Lk > 0x7fffff00;
 }
 
 bool bad_grid(long n) { return n <= 0 || n > 0x7fffffffL; }
+
+// A tile's rows lie within 31 bits of its first (DMA offsets), and (keys) none is masked out by itself.
+bool near(long a, long b) { return a < (1L << 23) && b < (1L << 23); }
+bool near_keys(const Att& p) { return !p.mask && near(p.vk.l, p.vv.l); }
+bool near_rows(const Att& p) {
+    return kStep % p.share == 0 && near(p.vq.l, p.vd.l) && near(p.vq.h * p.share / kStep, p.vd.h * p.share / kStep);
+}
 
 template <typename E, int DP> int launch_fwd(Att p, const Plan& n, hipStream_t st) {
     p.splits = n.fwd;
     const long blocks = n.fwd_groups * n.fwd, rows = (long)p.B * p.Hk * p.R;
     if (bad_grid(blocks) || bad_grid((rows + 3) / 4)) return -3;
     if constexpr (DP <= 64) {
-        if (n.nt == 2) xa_fwd_kernel<E, DP, 2><<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
+        if (n.nt == 2) {
+            const auto wide = near_keys(p) ? xa_fwd_kernel<E, DP, 2, true> : xa_fwd_kernel<E, DP, 2, false>;
+            wide<<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
+        }
     }
-    if (n.nt == 1) xa_fwd_kernel<E, DP, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
+    if (n.nt == 1) {
+        const auto kernel = near_keys(p) ? xa_fwd_kernel<E, DP, 1, true> : xa_fwd_kernel<E, DP, 1, false>;
+        kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
+    }
     if (n.fwd > 1) xa_join_kernel<E, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, rows);
     return DP_LAUNCH_STATUS();
 }
@@ -830,11 +901,13 @@ template <typename E, int DP> int launch_bwd(Att p, const Plan& n, hipStream_t s
         bad_grid((qn + 1023) / 1024))
         return -3;
     p.splits = n.dq;
-    xa_dq_kernel<E, DP><<<dim3((unsigned)(n.dq_groups * n.dq)), 256, 0, st>>>(p, n.dq_tiles);
+    const auto dq = near_keys(p) ? xa_dq_kernel<E, DP, true> : xa_dq_kernel<E, DP, false>;
+    const auto dkv = near_rows(p) ? xa_dkv_kernel<E, DP, true> : xa_dkv_kernel<E, DP, false>;
+    dq<<<dim3((unsigned)(n.dq_groups * n.dq)), 256, 0, st>>>(p, n.dq_tiles);
     if (n.dq > 1)
         xa_sum_kernel<E><<<dim3((unsigned)((qn + 1023) / 1024)), 256, 0, st>>>(p.part, qn, n.dq, qn, p.scale, (T*)p.dq);
     p.splits = n.dkv;
-    xa_dkv_kernel<E, DP><<<dim3((unsigned)(n.dkv_groups * n.dkv)), 256, 0, st>>>(p, n.ktiles);
+    dkv<<<dim3((unsigned)(n.dkv_groups * n.dkv)), 256, 0, st>>>(p, n.ktiles);
     if (n.dkv > 1) {
         const dim3 g((unsigned)((kv + 1023) / 1024));
         xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part, 2 * kv, n.dkv, kv, p.scale, (T*)p.dk);
