@@ -111,8 +111,8 @@ __device__ __forceinline__ float halves_sum(float v) {
 
 // Consecutive workgroups go round the 8 XCDs: give each XCD one contiguous range of the work, so that the workgroups
 // that read the same keys share an L2.
-__device__ __forceinline__ long xcd_order(long id, long total) {
-    const long x = id & 7, i = id >> 3, q = total >> 3, r = total & 7;
+__device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned total) {
+    const unsigned x = id & 7, i = id >> 3, q = total >> 3, r = total & 7;
     return x * q + (x < r ? x : r) + i;
 }
 
@@ -332,16 +332,14 @@ __device__ __forceinline__ void arrive() {
 
 struct Work { int b, hk, tile, split; };
 
-// work item: tiles fastest, then splits, then (image, key head)
+// Work item: tiles fastest, then splits, then (image, key head).  Scalars, so that what is addressed with them is too.
 __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
-    const long id = xcd_order(blockIdx.x, gridDim.x);
+    const unsigned id = xcd_order(blockIdx.x, gridDim.x), t = id / (unsigned)tiles, bh = t / (unsigned)p.splits;
     Work w;
-    w.tile = (int)(id % tiles);
-    const long t = id / tiles;
-    w.split = (int)(t % p.splits);
-    const long bh = t / p.splits;
-    w.hk = (int)(bh % p.Hk);
-    w.b = (int)(bh / p.Hk);
+    w.tile = __builtin_amdgcn_readfirstlane((int)(id - t * (unsigned)tiles));
+    w.split = __builtin_amdgcn_readfirstlane((int)(t - bh * (unsigned)p.splits));
+    w.b = __builtin_amdgcn_readfirstlane((int)(bh / (unsigned)p.Hk));
+    w.hk = __builtin_amdgcn_readfirstlane((int)(bh % (unsigned)p.Hk));
     return w;
 }
 
