@@ -142,17 +142,23 @@ __device__ __forceinline__ float row_max(const f32x16 (&s)[2]) {
     return mx;
 }
 
-// 64-bit set of the keys of block kb that take part; every wave of the workgroup gets the same set
-__device__ __forceinline__ unsigned long long key_set(const Att& p, int b, int len, int kb) {
-    if (!p.mask) {
+// 64-bit sets of the keys that take part, block after block; every wave of the workgroup gets the same.  A block's mask is
+// read one block before its set is asked for.
+struct KeySets {
+    const unsigned char* mask;
+    int len;
+    bool on;
+    __device__ __forceinline__ KeySets(const Att& p, int b, int n) { mask = p.mask ? p.mask + (long)b * p.mask_ld : nullptr; len = n; on = false; }
+    __device__ __forceinline__ void ahead(int kb) {
+        const int key = kb * 64 + (int)(threadIdx.x & 63);
+        if (mask) on = key < len && mask[key] != 0;
+    }
+    __device__ __forceinline__ unsigned long long of(int kb) const {       // kb: the block of the last ahead()
+        if (mask) return __ballot(on);
         const int left = len - kb * 64;
         return left >= 64 ? ~0ull : (1ull << left) - 1;
     }
-    const int key = kb * 64 + (int)(threadIdx.x & 63);
-    bool on = key < len;
-    if (on) on = p.mask[(long)b * p.mask_ld + key] != 0;
-    return __ballot(on);
-}
+};
 
 __device__ __forceinline__ int key_count(const Att& p, int b) {
     if (!p.lens) return p.Lk;
@@ -221,9 +227,9 @@ __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t from, unsigned char* 
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
 }
 
-// Successive tiles of rows, brought a tile ahead of their use.  DMA: straight into LDS, rows and columns that do not exist
-// as zeros; otherwise (masked keys, whose rows must become zeros whatever they hold; strides or head shares that do not
-// fit 32-bit offsets from a tile's first row) through registers.
+// Successive tiles of rows, brought a tile ahead of their use.  DMA: straight into LDS; rows and columns that do not exist,
+// and masked rows whatever they hold, come as zeros.  Otherwise (strides or head shares that do not fit 32-bit offsets from
+// a tile's first row) through registers.
 template <typename T, int DP, bool DMA> struct Stream {
     typedef Tile<DP> L;
     unsigned off[DMA ? L::kPieces : 1];
@@ -238,15 +244,16 @@ template <typename T, int DP, bool DMA> struct Stream {
             }
         }
     }
-    __device__ __forceinline__ void load(const T* tile, unsigned char* to, int rows) {
+    // `set`: the tile's rows that are read
+    __device__ __forceinline__ void load(const T* tile, unsigned char* to, unsigned long long set) {
         const __amdgpu_buffer_rsrc_t from = buffer_at(tile, 0x7fffffffu);
-        if (rows >= 64) {
+        if (set == ~0ull) {
 #pragma unroll
             for (int j = 0; j < L::kPieces; ++j) dma(from, to + (L::wave() * L::kPieces + j) * 1024, off[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < L::kPieces; ++j)
-                dma(from, to + (L::wave() * L::kPieces + j) * 1024, L::row(j) < rows ? off[j] : kOut);
+                dma(from, to + (L::wave() * L::kPieces + j) * 1024, set >> L::row(j) & 1 ? off[j] : kOut);
         }
     }
     __device__ __forceinline__ void put(unsigned char* to) const {
@@ -264,10 +271,10 @@ template <typename T, int DP, bool DMA> struct KeyStream : Stream<T, DP, DMA> {
         ld = v.l;
         this->open(p.D, ld, 0, 1);
     }
-    __device__ __forceinline__ void fetch(const Att& p, unsigned char* to, int kb, int len, unsigned long long set) {
+    __device__ __forceinline__ void fetch(const Att& p, unsigned char* to, int kb, unsigned long long set) {
         const T* tile = base + (long)kb * kKeys * ld;
         if constexpr (DMA) {
-            this->load(tile, to, len - kb * kKeys);
+            this->load(tile, to, set);
         } else {
 #pragma unroll
             for (int j = 0; j < L::kPieces; ++j) {
@@ -294,7 +301,8 @@ template <typename T, int DP, bool DMA> struct RowStream : Stream<T, DP, DMA> {
     }
     __device__ __forceinline__ void fetch(const Att& p, const View& v, int b, int hk, unsigned char* to, int st) {
         if constexpr (DMA) {
-            this->load(base + st * step, to, p.R - st * kStep);
+            const int left = p.R - st * kStep;
+            this->load(base + st * step, to, left >= 64 ? ~0ull : (1ull << left) - 1);
         } else {
 #pragma unroll
             for (int j = 0; j < L::kPieces; ++j) {
@@ -372,11 +380,14 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 4 : 2) void xa_fwd_kerne
     }
     const Reads<DP> rd;
     KeyStream<T, DP, DMA> ks_(p, p.k, p.vk, w.b, w.hk), vs_(p, p.v, p.vv, w.b, w.hk);
+    KeySets sets(p, w.b, len);
     unsigned long long set = 0, next = 0;
     if (kb0 < kb1) {
-        next = key_set(p, w.b, len, kb0);
-        ks_.fetch(p, K0, kb0, len, next);
-        vs_.fetch(p, V0, kb0, len, next);
+        sets.ahead(kb0);
+        next = sets.of(kb0);
+        ks_.fetch(p, K0, kb0, next);
+        vs_.fetch(p, V0, kb0, next);
+        sets.ahead(kb0 + 1);
     }
     // one block of keys from (kt, vt), the next on its way into (kn, vn)
     auto block = [&](unsigned char* kt, unsigned char* vt, unsigned char* kn, unsigned char* vn, int kb) {
@@ -387,9 +398,10 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 4 : 2) void xa_fwd_kerne
         set = next;
         arrive();                            // this block has landed; nobody reads (kn, vn) any more
         if (kb + 1 < kb1) {
-            next = key_set(p, w.b, len, kb + 1);
-            ks_.fetch(p, kn, kb + 1, len, next);
-            vs_.fetch(p, vn, kb + 1, len, next);
+            next = sets.of(kb + 1);
+            ks_.fetch(p, kn, kb + 1, next);
+            vs_.fetch(p, vn, kb + 1, next);
+            sets.ahead(kb + 2);
         }
         if (!wave_on || set == 0) return;
         f32x16 st[NT][2];
@@ -516,16 +528,23 @@ __global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
     const int r = (int)(id - bh * p.R);
     const float* base = p.part + (bh * p.splits * p.R + r) * (DP + 2);
     const long step = (long)p.R * (DP + 2);
-    float m = -kInf;
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, base[s * step + DP]);
-    const float mc = m == -kInf ? 0.f : m * p.c;
-    float l = 0.f, a0 = 0.f, a1 = 0.f;
+    // lane s weighs part s (at most 64 parts)
+    const float own = lane < p.splits ? base[lane * step + DP] : -kInf, sum = lane < p.splits ? base[lane * step + DP + 1] : 0.f;
+    float m = own;
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, k, 64));
+    const float f = m == -kInf ? 0.f : __builtin_amdgcn_exp2f((own - m) * p.c);
+    const float l = wave_sum(sum * f);
+    float a0 = 0.f, a1 = 0.f;
     const int d = lane * 2;
+#pragma unroll 8
     for (int s = 0; s < p.splits; ++s) {
-        const float* o = base + s * step;
-        const float f = __builtin_amdgcn_exp2f(fmaf(o[DP], p.c, -mc));
-        l = fmaf(o[DP + 1], f, l);
-        if (d < p.D) { a0 = fmaf(o[d], f, a0); a1 = fmaf(o[d + 1], f, a1); }
+        const float g = __shfl(f, s, 64);
+        if (d < DP) {
+            const float2 o = *reinterpret_cast<const float2*>(base + s * step + d);
+            a0 = fmaf(o.x, g, a0);
+            a1 = fmaf(o.y, g, a1);
+        }
     }
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     if (lane == 0 && p.lse) p.lse[id] = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : kInf;
@@ -583,11 +602,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
 
     const Reads<DP> rd;
     KeyStream<T, DP, DMA> ks_(p, p.k, p.vk, w.b, w.hk), vs_(p, p.v, p.vv, w.b, w.hk);
+    KeySets sets(p, w.b, len);
     unsigned long long set = 0, next = 0;
     if (kb0 < kb1) {
-        next = key_set(p, w.b, len, kb0);
-        ks_.fetch(p, K0, kb0, len, next);
-        vs_.fetch(p, V0, kb0, len, next);
+        sets.ahead(kb0);
+        next = sets.of(kb0);
+        ks_.fetch(p, K0, kb0, next);
+        vs_.fetch(p, V0, kb0, next);
+        sets.ahead(kb0 + 1);
     }
     auto block = [&](unsigned char* kt, unsigned char* vt, unsigned char* kn, unsigned char* vn, int kb) {
         if constexpr (!DMA) {
@@ -597,9 +619,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
         set = next;
         arrive();
         if (kb + 1 < kb1) {
-            next = key_set(p, w.b, len, kb + 1);
-            ks_.fetch(p, kn, kb + 1, len, next);
-            vs_.fetch(p, vn, kb + 1, len, next);
+            next = sets.of(kb + 1);
+            ks_.fetch(p, kn, kb + 1, next);
+            vs_.fetch(p, vn, kb + 1, next);
+            sets.ahead(kb + 2);
         }
         if (!wave_on || set == 0) return;
         // P (dP - delta) of 32 keys: keys on the registers, this lane's row
@@ -776,7 +799,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
         if (st + 1 < st1) block(Q1, D1, S1, Q0, D0, S0, st + 1);
     }
     if (key >= p.Lk) return;
-    const bool lone = len <= 64 && __popcll(key_set(p, w.b, len, 0)) == 1;
+    KeySets sets(p, w.b, len);
+    sets.ahead(0);
+    const bool lone = len > 0 && len <= 64 && __popcll(sets.of(0)) == 1;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) {
         if (!on) dv[t] = zero16();
@@ -853,10 +878,11 @@ Plan plan_of(int B, long R, int Lk, int Hk, int D) {
     n.fwd_groups = (long)B * Hk * n.fwd_tiles;
     n.dq_groups = (long)B * Hk * n.dq_tiles;
     n.dkv_groups = (long)B * Hk * n.ktiles;
-    const long keys = (Lk + kKeys - 1) / kKeys;
-    n.fwd = parts_for(n.fwd_groups, keys, 2 * kCus, 1.0);
-    n.dq = parts_for(n.dq_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, 1.0);
-    n.dkv = parts_for(n.dkv_groups, (R + kStep - 1) / kStep, (n.dp <= 64 ? 2 : 1) * kCus, 4.0);
+    // workgroups that a CU holds: registers for heads of 96 and more, LDS and registers for the rest
+    const long keys = (Lk + kKeys - 1) / kKeys, rows = (R + kStep - 1) / kStep;
+    n.fwd = parts_for(n.fwd_groups, keys, (n.dp <= 64 && n.nt == 1 ? 4 : 2) * kCus, 6.0);
+    n.dq = parts_for(n.dq_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, 6.0);
+    n.dkv = parts_for(n.dkv_groups, rows, (n.dp <= 64 ? 3 : 1) * kCus, 6.0);
     return n;
 }
 
@@ -867,9 +893,9 @@ bool bad(int B, int Lq, int Lk, int Hk, int share, int D) {
 
 bool bad_grid(long n) { return n <= 0 || n > 0x7fffffffL; }
 
-// A tile's rows lie within 31 bits of its first (DMA offsets), and (keys) none is masked out by itself.
+// A tile's rows lie within 31 bits of its first (DMA offsets).
 bool near(long a, long b) { return a < (1L << 23) && b < (1L << 23); }
-bool near_keys(const Att& p) { return !p.mask && near(p.vk.l, p.vv.l); }
+bool near_keys(const Att& p) { return near(p.vk.l, p.vv.l); }
 bool near_rows(const Att& p) {
     return kStep % p.share == 0 && near(p.vq.l, p.vd.l) && near(p.vq.h * p.share / kStep, p.vd.h * p.share / kStep);
 }
