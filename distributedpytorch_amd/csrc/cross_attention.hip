@@ -12,8 +12,8 @@
 // second operand of the product that contracts over them; the first operand of that product comes out of the row-major
 // LDS tile through transposing reads.
 //
-//   xa_fwd    128 or 256 rows a workgroup (32 or 64 a wave), keys in blocks of 64 through LDS, running maximum and sum;
-//             with few rows the keys are split over workgroups and xa_join puts the parts together
+//   xa_fwd    128 rows a workgroup (32 a wave), keys in blocks of 64 through LDS, running maximum and sum; with few rows
+//             the keys are split over workgroups and xa_join puts the parts together
 //   xa_dq     128 rows a workgroup, keys in blocks of 64; leaves delta behind for
 //   xa_dkv    128 keys a workgroup (32 a wave, their k and v in registers), rows in blocks of 64 through LDS
 //   xa_sum    joins the fp32 parts of dq, or of dk and dv, where a long axis was split; one order, no atomics
@@ -352,32 +352,26 @@ __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// NT: row tiles of 32 of a wave.
-template <typename E, int DP, int NT, bool DMA>
-__global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, int tiles) {
+template <typename E, int DP, bool DMA>
+__global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, int tiles) {
     typedef typename E::raw T;
     // (four variables, not an array: the compiler then knows that what is brought into one is not what is read)
     __shared__ __attribute__((aligned(16))) unsigned char K0[Tile<DP>::kBytes], V0[Tile<DP>::kBytes], K1[Tile<DP>::kBytes],
         V1[Tile<DP>::kBytes];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
     const Work w = work_of(p, tiles);
-    const int r0 = w.tile * (kRows * NT) + wave * (32 * NT) + l31;
-    const bool wave_on = r0 - l31 < p.R;
+    const int r = w.tile * kRows + wave * 32 + l31;
+    const bool row_on = r < p.R, wave_on = r - l31 < p.R;
     const int len = key_count(p, w.b);
     const int nkb = (len + kKeys - 1) / kKeys;
     const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
 
-    uint4 qf[NT][DP / 16];
-    f32x16 acc[NT][DP / 32];
-    float m[NT], l[NT];
+    uint4 qf[DP / 16];
+    row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r, row_on, qf);
+    f32x16 acc[DP / 32];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r0 + 32 * n, r0 + 32 * n < p.R, qf[n]);
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t) acc[n][t] = zero16();
-        m[n] = -kInf;
-        l[n] = 0.f;
-    }
+    for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
+    float m = -kInf, l = 0.f;
     const Reads<DP> rd;
     KeyStream<T, DP, DMA> ks_(p, p.k, p.vk, w.b, w.hk), vs_(p, p.v, p.vv, w.b, w.hk);
     KeySets sets(p, w.b, len);
@@ -404,117 +398,85 @@ __global__ __launch_bounds__(256, NT == 1 && DP <= 64 ? 4 : 2) void xa_fwd_kerne
             sets.ahead(kb + 2);
         }
         if (!wave_on || set == 0) return;
-        f32x16 st[NT][2];
-        float top[NT], mc[NT];
-        uint4 pf[NT][4];
-        auto probabilities = [&](int n) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                f32x16& x = st[n][s >> 1];
-#pragma unroll
-                for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) {
-                    x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, -mc[n]));
-                    l[n] += x[i];
-                }
-                pf[n][s] = pack_acc<E>(x, s & 1);
-            }
-        };
-        // S^T: keys on the registers, this lane's rows
-#pragma unroll
-        for (int n = 0; n < NT; ++n) st[n][0] = st[n][1] = zero16();
+        // S^T: keys on the registers, this lane's row
+        f32x16 st[2] = {zero16(), zero16()};
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint4 kf = rd.rows(kt, t, ks);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) st[n][t] = E::mfma(kf, qf[n][ks], st[n][t]);
-            }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) top[n] = row_max(st[n]);
+            for (int t = 0; t < 2; ++t) st[t] = E::mfma(rd.rows(kt, t, ks), qf[ks], st[t]);
+        float top = row_max(st);
         if (set != ~0ull) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) st[n][t][i] = (bits >> entry(i, 0) & 1) ? st[n][t][i] : -kInf;
+                for (int i = 0; i < 16; ++i) st[t][i] = (bits >> entry(i, 0) & 1) ? st[t][i] : -kInf;
             }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) top[n] = row_max(st[n]);
+            top = row_max(st);
         }
-        bool rises = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            top[n] = halves_max(top[n]);
-            rises |= !(top[n] * p.c <= fmaf(m[n], p.c, 8.f));
-        }
+        top = halves_max(top);
         // The reference m only follows the maximum where it is passed by more than 2^8: probabilities relative to it stay
         // far inside both types' range, and the accumulators are seldom rescaled.
-        if (__any(rises)) {
+        if (__any(!(top * p.c <= fmaf(m, p.c, 8.f)))) {
+            const float up = __builtin_elementwise_maximum(m, top);
+            const float alpha = up == -kInf ? 1.f : __builtin_amdgcn_exp2f((m - up) * p.c);   // (m = -inf: 0)
+            l *= alpha;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float up = __builtin_elementwise_maximum(m[n], top[n]);
-                const float alpha = up == -kInf ? 1.f : __builtin_amdgcn_exp2f((m[n] - up) * p.c);   // (m = -inf: 0)
-                l[n] *= alpha;
+            for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-                for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[n][t][i] *= alpha;
-                m[n] = up;
-            }
+                for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+            m = up;
         }
+        const float mc = m == -kInf ? 0.f : m * p.c;
+        uint4 pf[4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mc[n] = m[n] == -kInf ? 0.f : m[n] * p.c;
+        for (int s = 0; s < 4; ++s) {
+            f32x16& x = st[s >> 1];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) probabilities(n);
+            for (int i = 8 * (s & 1); i < 8 * (s & 1) + 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, -mc));
+                l += x[i];
+            }
+            pf[s] = pack_acc<E>(x, s & 1);
+        }
         // O^T += V^T P^T
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t) {
-                const uint4 vf = rd.cols(vt, s, t);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) acc[n][t] = E::mfma(vf, pf[n][s], acc[n][t]);
-            }
+            for (int t = 0; t < DP / 32; ++t) acc[t] = E::mfma(rd.cols(vt, s, t), pf[s], acc[t]);
     };
     for (int kb = kb0; kb < kb1; kb += 2) {
         block(K0, V0, K1, V1, kb);
         if (kb + 1 < kb1) block(K1, V1, K0, V0, kb + 1);
     }
     const long bh = (long)w.b * p.Hk + w.hk;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = r0 + 32 * n;
-        const float sum = halves_sum(l[n]);
-        if (r >= p.R) continue;
-        if (p.splits > 1) {
-            float* o = p.part + ((bh * p.splits + w.split) * p.R + r) * (DP + 2);
-            if (h == 0) { o[DP] = m[n]; o[DP + 1] = sum; }
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                    *reinterpret_cast<float2*>(o + t * 32 + entry(i, h)) = make_float2(acc[n][t][i], acc[n][t][i + 1]);
-            continue;
-        }
-        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-        if (h == 0 && p.lse) p.lse[bh * p.R + r] = sum > 0.f ? fmaf(m[n], p.c, __builtin_amdgcn_logf(sum)) : kInf;
-        T* o = (T*)p.out + dense_row(p, w.b, w.hk, r);
+    l = halves_sum(l);
+    if (!row_on) return;
+    if (p.splits > 1) {
+        float* o = p.part + ((bh * p.splits + w.split) * p.R + r) * (DP + 2);
+        if (h == 0) { o[DP] = m; o[DP + 1] = l; }
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int d = t * 32 + 8 * g + 4 * h;
-                if (d < p.D) {
-                    uint2 u;
-                    u.x = E::pair(acc[n][t][4 * g] * inv, acc[n][t][4 * g + 1] * inv);
-                    u.y = E::pair(acc[n][t][4 * g + 2] * inv, acc[n][t][4 * g + 3] * inv);
-                    *reinterpret_cast<uint2*>(o + d) = u;
-                }
-            }
+            for (int i = 0; i < 16; i += 2)
+                *reinterpret_cast<float2*>(o + t * 32 + entry(i, h)) = make_float2(acc[t][i], acc[t][i + 1]);
+        return;
     }
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    if (h == 0 && p.lse) p.lse[bh * p.R + r] = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : kInf;
+    T* o = (T*)p.out + dense_row(p, w.b, w.hk, r);
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = t * 32 + 8 * g + 4 * h;
+            if (d < p.D) {
+                uint2 u;
+                u.x = E::pair(acc[t][4 * g] * inv, acc[t][4 * g + 1] * inv);
+                u.y = E::pair(acc[t][4 * g + 2] * inv, acc[t][4 * g + 3] * inv);
+                *reinterpret_cast<uint2*>(o + d) = u;
+            }
+        }
 }
 
 // joins the splits of one row: a wave per row
@@ -866,23 +828,20 @@ int parts_for(long groups, long steps, long slots, double extra) {
 
 constexpr long kCus = 256;
 
-struct Plan { long fwd_groups, dq_groups, dkv_groups; int fwd_tiles, dq_tiles, ktiles, nt, fwd, dkv, dq, dp; };
+struct Plan { long row_groups, key_groups; int rtiles, ktiles, fwd, dkv, dq, dp; };
 
 Plan plan_of(int B, long R, int Lk, int Hk, int D) {
     Plan n;
     n.dp = padded(D);
-    n.nt = n.dp < 64 && R > kRows ? 2 : 1;
-    n.fwd_tiles = (int)((R + kRows * n.nt - 1) / (kRows * n.nt));
-    n.dq_tiles = (int)((R + kRows - 1) / kRows);
+    n.rtiles = (int)((R + kRows - 1) / kRows);
     n.ktiles = (Lk + kRows - 1) / kRows;
-    n.fwd_groups = (long)B * Hk * n.fwd_tiles;
-    n.dq_groups = (long)B * Hk * n.dq_tiles;
-    n.dkv_groups = (long)B * Hk * n.ktiles;
+    n.row_groups = (long)B * Hk * n.rtiles;
+    n.key_groups = (long)B * Hk * n.ktiles;
     // workgroups that a CU holds: registers for heads of 96 and more, LDS and registers for the rest
     const long keys = (Lk + kKeys - 1) / kKeys, rows = (R + kStep - 1) / kStep;
-    n.fwd = parts_for(n.fwd_groups, keys, (n.dp <= 64 && n.nt == 1 ? 4 : 2) * kCus, 6.0);
-    n.dq = parts_for(n.dq_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, 6.0);
-    n.dkv = parts_for(n.dkv_groups, rows, (n.dp <= 64 ? 3 : 1) * kCus, 6.0);
+    n.fwd = parts_for(n.row_groups, keys, (n.dp <= 64 ? 4 : 2) * kCus, 6.0);
+    n.dq = parts_for(n.row_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, 6.0);
+    n.dkv = parts_for(n.key_groups, rows, (n.dp <= 64 ? 3 : 1) * kCus, 6.0);
     return n;
 }
 
@@ -902,18 +861,10 @@ bool near_rows(const Att& p) {
 
 template <typename E, int DP> int launch_fwd(Att p, const Plan& n, hipStream_t st) {
     p.splits = n.fwd;
-    const long blocks = n.fwd_groups * n.fwd, rows = (long)p.B * p.Hk * p.R;
+    const long blocks = n.row_groups * n.fwd, rows = (long)p.B * p.Hk * p.R;
     if (bad_grid(blocks) || bad_grid((rows + 3) / 4)) return -3;
-    if constexpr (DP <= 64) {
-        if (n.nt == 2) {
-            const auto wide = near_keys(p) ? xa_fwd_kernel<E, DP, 2, true> : xa_fwd_kernel<E, DP, 2, false>;
-            wide<<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
-        }
-    }
-    if (n.nt == 1) {
-        const auto kernel = near_keys(p) ? xa_fwd_kernel<E, DP, 1, true> : xa_fwd_kernel<E, DP, 1, false>;
-        kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.fwd_tiles);
-    }
+    const auto kernel = near_keys(p) ? xa_fwd_kernel<E, DP, true> : xa_fwd_kernel<E, DP, false>;
+    kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.rtiles);
     if (n.fwd > 1) xa_join_kernel<E, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, rows);
     return DP_LAUNCH_STATUS();
 }
@@ -921,17 +872,17 @@ template <typename E, int DP> int launch_fwd(Att p, const Plan& n, hipStream_t s
 template <typename E, int DP> int launch_bwd(Att p, const Plan& n, hipStream_t st) {
     typedef typename E::raw T;
     const long kv = (long)p.B * p.Lk * p.Hk * p.D, qn = (long)p.B * p.Hk * p.R * p.D;
-    if (bad_grid(n.dkv_groups * n.dkv) || bad_grid(n.dq_groups * n.dq) || bad_grid((kv + 1023) / 1024) ||
+    if (bad_grid(n.key_groups * n.dkv) || bad_grid(n.row_groups * n.dq) || bad_grid((kv + 1023) / 1024) ||
         bad_grid((qn + 1023) / 1024))
         return -3;
     p.splits = n.dq;
     const auto dq = near_keys(p) ? xa_dq_kernel<E, DP, true> : xa_dq_kernel<E, DP, false>;
     const auto dkv = near_rows(p) ? xa_dkv_kernel<E, DP, true> : xa_dkv_kernel<E, DP, false>;
-    dq<<<dim3((unsigned)(n.dq_groups * n.dq)), 256, 0, st>>>(p, n.dq_tiles);
+    dq<<<dim3((unsigned)(n.row_groups * n.dq)), 256, 0, st>>>(p, n.rtiles);
     if (n.dq > 1)
         xa_sum_kernel<E><<<dim3((unsigned)((qn + 1023) / 1024)), 256, 0, st>>>(p.part, qn, n.dq, qn, p.scale, (T*)p.dq);
     p.splits = n.dkv;
-    dkv<<<dim3((unsigned)(n.dkv_groups * n.dkv)), 256, 0, st>>>(p, n.ktiles);
+    dkv<<<dim3((unsigned)(n.key_groups * n.dkv)), 256, 0, st>>>(p, n.ktiles);
     if (n.dkv > 1) {
         const dim3 g((unsigned)((kv + 1023) / 1024));
         xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part, 2 * kv, n.dkv, kv, p.scale, (T*)p.dk);
