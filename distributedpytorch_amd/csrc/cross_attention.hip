@@ -110,7 +110,7 @@ __device__ __forceinline__ float halves_sum(float v) {
 }
 
 // Consecutive workgroups go round the 8 XCDs: give each XCD one contiguous range of the work, so that the workgroups
-// that read the same keys share an L2.
+// that read the same keys share an L2.  Not with lengths: an XCD would get the long images whole, another the empty ones.
 __device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned total) {
     const unsigned x = id & 7, i = id >> 3, q = total >> 3, r = total & 7;
     return x * q + (x < r ? x : r) + i;
@@ -342,7 +342,7 @@ struct Work { int b, hk, tile, split; };
 
 // Work item: tiles fastest, then splits, then (image, key head).  Scalars, so that what is addressed with them is too.
 __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
-    const unsigned id = xcd_order(blockIdx.x, gridDim.x), t = id / (unsigned)tiles, bh = t / (unsigned)p.splits;
+    const unsigned id = p.lens ? blockIdx.x : xcd_order(blockIdx.x, gridDim.x), t = id / (unsigned)tiles, bh = t / (unsigned)p.splits;
     Work w;
     w.tile = __builtin_amdgcn_readfirstlane((int)(id - t * (unsigned)tiles));
     w.split = __builtin_amdgcn_readfirstlane((int)(t - bh * (unsigned)p.splits));
