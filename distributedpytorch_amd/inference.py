@@ -267,14 +267,17 @@ class InstancePredictor(_Base):
 
 
 def load_predictor(task: str, model_name: str, weights: Optional[str] = None, num_classes: Optional[int] = None,
-                   output_stride: Optional[int] = None, device=None, **kw):
+                   output_stride: Optional[int] = None, device=None, norm: str = "batch", decoder_attention: bool = False,
+                   **kw):
     """Model by name (+ a checkpoint written by this framework or by the reference: utils.checkpoint.load_weights) in
-    the predictor of ``task`` ('semseg' | 'instance')."""
+    the predictor of ``task`` ('semseg' | 'instance'); ``norm`` / ``decoder_attention`` as the model was trained
+    (``models.build_model``)."""
     from .models import build_model
     from .utils.checkpoint import load_weights
     instance = task == "instance"
     nclass = num_classes if num_classes is not None else (1 if instance else 21)
-    model = build_model(model_name, nclass, output_stride=output_stride, in_channels=4 if instance else 3)
+    model = build_model(model_name, nclass, output_stride=output_stride, in_channels=4 if instance else 3, norm=norm,
+                        decoder_attention=decoder_attention)
     if weights:
         load_weights(weights, model, strict=True)
     cls = InstancePredictor if instance else SemSegPredictor

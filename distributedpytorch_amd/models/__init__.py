@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch.nn as nn
 
-from ..ops import convert_sync_batchnorm, freeze_batchnorm
+from ..ops import convert_group_norm, convert_sync_batchnorm, freeze_batchnorm
 from .danet import DANet
 from .deeplab import ASPP, Decoder, DeepLabV3Plus
 from .fcn import FCN
@@ -29,21 +29,34 @@ _ALIASES = {
 
 def build_model(name: str = "deeplabv3plus_resnet101", num_classes: int = 21, output_stride: int | None = None,
                 sync_bn: bool = False, freeze_bn: bool = False, in_channels: int = 3,
-                process_group=None) -> nn.Module:
+                process_group=None, norm: str = "batch", decoder_attention: bool = False) -> nn.Module:
     """Construct a segmentation network by name.
 
     ``sync_bn`` / ``freeze_bn`` mirror the knobs of the reference's commented DeepLab constructor
-    (`/root/reference/train_pascal.py:85`)."""
+    (`/root/reference/train_pascal.py:85`).  ``norm``: ``'batch'``, or ``'group'`` for group norm in every layer's place
+    (statistics of one image: training at a few images per GPU; ResNet backbones).  ``decoder_attention``: DeepLabv3+
+    with cross attention from the decoder's positions to the encoder's map (``models.deeplab.DecoderAttention``)."""
     name = _ALIASES.get(name, name)
     head, _, backbone = name.partition("_")
+    if norm not in ("batch", "group"):
+        raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+    if norm == "group" and (sync_bn or freeze_bn):
+        raise ValueError("sync_bn / freeze_bn are about batch statistics: group norm has none")
+    if norm == "group" and backbone.startswith("xception"):
+        raise NotImplementedError("Xception's middle flow is stored wider than it is: its zero channels would enter a group's "
+                                  "statistics (norm='group' takes the ResNet backbones)")
+    if decoder_attention and head != "deeplabv3plus":
+        raise ValueError("decoder_attention: DeepLabv3+ models")
     if head == "fcn":
         model = FCN(num_classes, backbone, output_stride or 32, in_channels)
     elif head == "deeplabv3plus":
-        model = DeepLabV3Plus(num_classes, backbone, output_stride or 16, in_channels)
+        model = DeepLabV3Plus(num_classes, backbone, output_stride or 16, in_channels, decoder_attention)
     elif head == "danet":
         model = DANet(num_classes, backbone, in_channels, output_stride or 8)
     else:
         raise ValueError(f"unknown model '{name}'; choose from {MODEL_NAMES}")
+    if norm == "group":
+        convert_group_norm(model)
     if sync_bn:
         convert_sync_batchnorm(model, process_group)
     if freeze_bn:

@@ -16,7 +16,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops import conv_bn_act, BatchNorm2d, Conv2d, GlobalAvgPool, bilinear_resize
+from ..ops import (BatchNorm2d, Conv2d, GlobalAvgPool, GroupNorm2d, bilinear_resize, conv_bn_act, cross_attention,
+                   dropout)
 from ..ops.concat import ChannelConcat
 from .resnet import ResNet
 from .xception import AlignedXception
@@ -100,15 +101,48 @@ class _LastConv(nn.Module):
         return getattr(self, "8")(x, sole_consumer=True)
 
 
+class DecoderAttention(nn.Module):
+    """``up + dropout(GN(project(attention)))``: every stride-4 position of the low-level map asks the pyramid's map at
+    the encoder's stride, instead of only taking what bilinear interpolation puts there.  ``GN``'s weight starts at
+    zero, so the decoder starts as the one without attention."""
+
+    def __init__(self, low_channels: int, channels: int, heads: int = 4, dropout: float = 0.1):
+        super().__init__()
+        self.heads, self.p_drop = heads, dropout
+        self.query_conv = Conv2d(low_channels, channels, 1)
+        self.key_value_conv = Conv2d(channels, 2 * channels, 1)
+        self.project = Conv2d(channels, channels, 1, bias=False)
+        self.norm = GroupNorm2d(channels, 32)
+        nn.init.zeros_(self.norm.weight)
+
+    def _sequence(self, t):                    # [N, C, H, W] -> [N, H W, heads, C / heads]: a view of a channels-last map
+        n, c, h, w = t.shape
+        return t.permute(0, 2, 3, 1).reshape(n, h * w, self.heads, c // self.heads)
+
+    def forward(self, low, context, up):
+        n, _, h, w = low.shape
+        kv = self.key_value_conv(context)
+        c = kv.shape[1] // 2
+        y = cross_attention(self._sequence(self.query_conv(low)), self._sequence(kv[:, :c]), self._sequence(kv[:, c:]))
+        y = self.norm(self.project(y.reshape(n, h, w, c).permute(0, 3, 1, 2)))
+        return dropout(y, self.p_drop, self.training, residual=up)
+
+
 class Decoder(nn.Module):
-    def __init__(self, low_level_channels: int, num_classes: int):
+    def __init__(self, low_level_channels: int, num_classes: int, attention: bool = False):
         super().__init__()
         self.conv1 = Conv2d(low_level_channels, 48, 1, bias=False)
         self.bn1 = BatchNorm2d(48)
         self.last_conv = _LastConv(256 + 48, num_classes)
+        if attention:
+            self.attention = DecoderAttention(48, 256)
 
     def forward(self, x, low):
         size = low.shape[2:]
+        if hasattr(self, "attention"):
+            low = conv_bn_act(self.conv1, self.bn1, low, relu=True)
+            up = bilinear_resize(x, size) if tuple(x.shape[2:]) != tuple(size) else x
+            return self.last_conv(torch.cat((self.attention(low, x, up), low), dim=1), self.training)
         cc = ChannelConcat(x, (x.shape[1], self.conv1.out_channels), size)
         if tuple(x.shape[2:]) == tuple(size):
             cc.in_place = False                       # nothing to resize: no producer to write slot 0
@@ -119,7 +153,7 @@ class Decoder(nn.Module):
 
 class DeepLabV3Plus(nn.Module):
     def __init__(self, num_classes: int = 21, backbone: str = "resnet101", output_stride: int = 16,
-                 in_channels: int = 3):
+                 in_channels: int = 3, decoder_attention: bool = False):
         super().__init__()
         if backbone.startswith("resnet"):
             self.backbone = ResNet(backbone, output_stride, in_channels)
@@ -128,7 +162,7 @@ class DeepLabV3Plus(nn.Module):
         else:
             raise ValueError(f"unknown backbone {backbone}")
         self.aspp = ASPP(self.backbone.out_channels, output_stride)
-        self.decoder = Decoder(self.backbone.low_level_channels, num_classes)
+        self.decoder = Decoder(self.backbone.low_level_channels, num_classes, decoder_attention)
         self.num_classes = num_classes
         # When set (by the training engine, for a criterion that upsamples inside the loss kernel:
         # ops.loss / csrc/upsample_ce.hip) the training forward returns the stride-4 logits and the

@@ -12,7 +12,7 @@ from .bnfold import conv_bn_add_relu  # noqa: F401
 from .conv import Conv2d, conv2d, conv_bn_act, conv_out_size  # noqa: F401
 from .cross_attention import cross_attention  # noqa: F401
 from .dropout import dropout  # noqa: F401
-from .group_norm import group_norm_act  # noqa: F401
+from .group_norm import GroupNorm2d, convert_group_norm, group_norm_act  # noqa: F401
 from .loss import SoftmaxCrossEntropy, softmax_cross_entropy  # noqa: F401
 from .metrics import confusion_matrix, miou_from_confusion  # noqa: F401
 from .pool import GlobalAvgPool, MaxPool3x3s2, global_avg_pool, max_pool3x3s2  # noqa: F401

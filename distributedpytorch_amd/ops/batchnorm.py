@@ -405,6 +405,8 @@ class BatchNorm2d(nn.Module):
     ``sync`` turns on cross-rank statistics (SyncBatchNorm); ``frozen`` uses running statistics
     even in training mode (the reference's ``freeze_bn``)."""
 
+    batch_statistics = True        # (ops.group_norm.GroupNorm2d, which can stand in its place, has none)
+
     def __init__(self, num_features: int, eps: float = 1e-5, momentum: float = 0.1,
                  sync: bool = False, frozen: bool = False, process_group=None):
         super().__init__()

@@ -206,7 +206,7 @@ class _ConvBnAddReluFold(torch.autograd.Function):
 
 def can_fold(conv, bn, x: torch.Tensor, residual: Optional[torch.Tensor]) -> bool:
     return (_ENABLED and B.use_hip(x) and x.dtype == torch.bfloat16 and torch.is_grad_enabled()
-            and residual is not None and bn.training and not bn.frozen and bn.weight is not None
+            and residual is not None and bn.batch_statistics and bn.training and not bn.frozen and bn.weight is not None
             and conv.kernel_size == (1, 1) and conv.stride == (1, 1) and conv.padding == (0, 0)
             and conv.groups == 1 and conv.bias is None and conv.in_channels % 8 == 0 and conv.out_channels % 8 == 0
             and tuple(residual.shape) == (x.shape[0], conv.out_channels, x.shape[2], x.shape[3])

@@ -159,7 +159,8 @@ def _infer_fused(conv: "Conv2d", bn, x: torch.Tensor, relu: bool, residual: Opti
 def conv_bn_act(conv: "Conv2d", bn, x: torch.Tensor, relu: bool = False,
                 residual: Optional[torch.Tensor] = None, passthrough: bool = False, sole_consumer: bool = False,
                 dropout: float = 0.0, out=None):
-    """``act(BN(conv(x)) + residual)``.  On the GPU path the batch statistics come out of the conv
+    """``act(BN(conv(x)) + residual)``; ``bn``: a ``BatchNorm2d``, or a ``GroupNorm2d`` in its place (run behind the
+    convolution, nothing fused into it).  On the GPU path the batch statistics come out of the conv
     kernel's epilogue (no separate statistics pass over the activation).
 
     ``dropout``: probability of a dropout behind the activation (training only), run inside the BN
@@ -172,7 +173,7 @@ def conv_bn_act(conv: "Conv2d", bn, x: torch.Tensor, relu: bool = False,
     autograd node: use ``x'`` as the block's identity and the skip-path gradient is added inside the
     data-gradient kernel (csrc/conv_igemm2.hip store loop) instead of by an add kernel."""
     slot = out
-    if (INFER_FUSE and not bn.training and slot is None and not torch.is_grad_enabled() and B.use_hip(x)
+    if (INFER_FUSE and bn.batch_statistics and not bn.training and slot is None and not torch.is_grad_enabled() and B.use_hip(x)
             and x.dtype == torch.bfloat16 and conv.groups == 1 and conv.bias is None
             and conv.stride[0] == conv.stride[1] and conv.in_channels % 8 == 0 and conv.out_channels % 8 == 0):
         # evaluation: BatchNorm (running statistics), identity add and ReLU in the convolution's epilogue
@@ -180,7 +181,7 @@ def conv_bn_act(conv: "Conv2d", bn, x: torch.Tensor, relu: bool = False,
         if y is not None:
             return (y, x) if passthrough else y
     pt = passthrough and conv.can_passthrough(x)
-    if bn.training and not bn.frozen and conv.can_fuse_stats(x):
+    if bn.batch_statistics and bn.training and not bn.frozen and conv.can_fuse_stats(x):
         if pt:
             y, stats, skip = conv(x, with_stats=True, passthrough=True, sole_consumer=sole_consumer)
         else:

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from typing import Optional
 
 import torch
@@ -178,3 +179,48 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, code)
     return _forward(x, num_groups, _vec(weight), _vec(bias), eps, code, residual)[0]
+
+
+class GroupNorm2d(nn.Module):
+    """``nn.GroupNorm``-compatible parameters; forward takes ``BatchNorm2d``'s fusion flags, so that it stands where a
+    ``BatchNorm2d`` does (``ops.conv_bn_act``): ``forward(x, relu, residual, dropout=p)`` is
+    ``dropout(act(GN(x) + residual))``, dropout in training mode only."""
+
+    batch_statistics = False       # nothing for a convolution's epilogue to collect, nothing to fold or to synchronise
+    frozen = False
+
+    def __init__(self, num_features: int, num_groups: int = 32, eps: float = 1e-5):
+        super().__init__()
+        if num_groups <= 0 or num_features % num_groups:
+            raise ValueError(f"GroupNorm2d: {num_features} channels do not split into {num_groups} groups")
+        self.num_features, self.num_groups, self.eps = num_features, num_groups, eps
+        self.weight = nn.Parameter(torch.ones(num_features))
+        self.bias = nn.Parameter(torch.zeros(num_features))
+
+    def forward(self, x: torch.Tensor, relu: bool = False, residual: Optional[torch.Tensor] = None, stats=None,
+                dropout: float = 0.0, out=None):
+        """``stats`` and ``out`` (a convolution's sums, a concat slot) are ``BatchNorm2d``'s and have no use here: the
+        result is an ordinary tensor, which ``ops.concat`` copies."""
+        y = group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, "relu" if relu else None, residual)
+        if dropout > 0.0 and self.training:
+            from .dropout import dropout as _dropout
+            y = _dropout(y, dropout)
+        return y
+
+    def extra_repr(self) -> str:
+        return f"{self.num_features}, num_groups={self.num_groups}, eps={self.eps}"
+
+
+def convert_group_norm(module: nn.Module, num_groups: int = 32) -> nn.Module:
+    """Replace every ``BatchNorm2d`` in ``module`` by a ``GroupNorm2d`` of the same weight and bias (in place), with
+    the largest number of groups that divides both ``num_groups`` and its channels."""
+    from .batchnorm import BatchNorm2d
+    for name, child in module.named_children():
+        if isinstance(child, BatchNorm2d):
+            gn = GroupNorm2d(child.num_features, math.gcd(num_groups, child.num_features), child.eps)
+            gn.weight, gn.bias = child.weight, child.bias
+            gn.train(child.training)
+            setattr(module, name, gn)
+        else:
+            convert_group_norm(child, num_groups)
+    return module

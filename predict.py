@@ -38,6 +38,8 @@ def parse_args(argv=None):
     ap.add_argument("--weights", default=None, help="checkpoint (.pth); without it the weights are random (a rate run)")
     ap.add_argument("--num-classes", type=int, default=None)
     ap.add_argument("--output-stride", type=int, default=None)
+    ap.add_argument("--norm", choices=["batch", "group"], default="batch", help="as the model was trained")
+    ap.add_argument("--decoder-attention", action="store_true", help="as the model was trained")
     ap.add_argument("--input", default=None, help="an image, a directory of images or a glob pattern")
     ap.add_argument("--output", default="predictions")
     ap.add_argument("--points", default=None, help="instance task: 'x,y x,y x,y x,y' per image, groups separated by ';'")
@@ -115,7 +117,8 @@ def main(argv=None):
         rank, world, device = info.rank, info.world_size, info.device
     else:
         device = torch.device("cpu") if args.cpu or not torch.cuda.is_available() else torch.device("cuda", 0)
-    kw = dict(crop=crop, batch=args.batch, graph=not args.no_graph)
+    kw = dict(crop=crop, batch=args.batch, graph=not args.no_graph, norm=args.norm,
+              decoder_attention=args.decoder_attention)
     if not instance:
         kw["fit"] = args.fit
     torch.manual_seed(0)

@@ -81,6 +81,10 @@ def parse_args(argv=None):
     ap.add_argument("--crop", type=int, default=None, help="513 (semseg) / 512 (instance)")
     ap.add_argument("--sync-bn", action="store_true")
     ap.add_argument("--freeze-bn", action="store_true")
+    ap.add_argument("--norm", choices=["batch", "group"], default="batch",
+                    help="group: group norm in every layer's place (a few images per GPU; ResNet backbones)")
+    ap.add_argument("--decoder-attention", action="store_true",
+                    help="DeepLabv3+ with cross attention from the decoder's positions to the encoder's map")
     ap.add_argument("--head-lr-mult", type=float, default=1.0, help="10 = the 1x/10x groups of train_pascal.py:90-91")
     ap.add_argument("--lr-mode", choices=["poly", "cos", "step", "const"], default=None)
     ap.add_argument("--synthetic", action="store_true", help="VOC-shaped random data (no dataset on disk)")
@@ -514,7 +518,8 @@ def main(argv=None):
 
     nclass = 1 if instance else 21
     net = build_model(args.model, nclass, output_stride=args.output_stride, sync_bn=args.sync_bn,
-                      freeze_bn=args.freeze_bn, in_channels=args.nInputChannels)
+                      freeze_bn=args.freeze_bn, in_channels=args.nInputChannels, norm=args.norm,
+                      decoder_attention=args.decoder_attention)
     if info.is_master:
         n_params = sum(p.numel() for p in net.parameters() if p.requires_grad)
         backbone = getattr(net, "backbone", None)
