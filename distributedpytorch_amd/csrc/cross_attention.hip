@@ -45,10 +45,6 @@ struct Bf {
     static __device__ __forceinline__ void unpair(unsigned u, float& lo, float& hi) {
         lo = __uint_as_float(u << 16); hi = __uint_as_float(u & 0xffff0000u);
     }
-    // c + both halves of u
-    static __device__ __forceinline__ float add_pair(unsigned u, float c) {
-        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u), (bf16x2){(__bf16)1.f, (__bf16)1.f}, c, false);
-    }
 };
 
 struct Hf {
@@ -61,9 +57,6 @@ struct Hf {
     }
     static __device__ __forceinline__ void unpair(unsigned u, float& lo, float& hi) {
         lo = (float)__builtin_bit_cast(f16, (unsigned short)u); hi = (float)__builtin_bit_cast(f16, (unsigned short)(u >> 16));
-    }
-    static __device__ __forceinline__ float add_pair(unsigned u, float c) {
-        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, u), (f16x2){(f16)1.f, (f16)1.f}, c, false);
     }
 };
 
@@ -89,6 +82,11 @@ struct Att {
     int splits;                      // parts of the split axis
     float* part;                     // their fp32 partial results
 };
+
+// A row's log2 of the sum l of its exponentials relative to m: +inf without a key (P = 0 in backward), NaN stays NaN.
+__device__ __forceinline__ float log_sum(float m, float l, float c) {
+    return l > 0.f ? fmaf(m, c, __builtin_amdgcn_logf(l)) : (l == l ? kInf : l);
+}
 
 __device__ __forceinline__ f32x16 splat16(float v) {
     f32x16 z;
@@ -463,7 +461,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, in
         return;
     }
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    if (h == 0 && p.lse) p.lse[bh * p.R + r] = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : kInf;
+    if (h == 0 && p.lse) p.lse[bh * p.R + r] = log_sum(m, l, p.c);
     T* o = (T*)p.out + dense_row(p, w.b, w.hk, r);
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -509,7 +507,7 @@ __global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
         }
     }
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    if (lane == 0 && p.lse) p.lse[id] = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : kInf;
+    if (lane == 0 && p.lse) p.lse[id] = log_sum(m, l, p.c);
     if (d < p.D) {
         const int b = (int)(bh / p.Hk), hk = (int)(bh % p.Hk);
         T* o = (T*)p.out + dense_row(p, b, hk, r);

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __re
                                                             const T* __restrict__ res, const float* __restrict__ w,
                                                             const float* __restrict__ b,
                                                             const double* __restrict__ stats, float* __restrict__ part) {
-    constexpr bool kExact = sizeof(T) == 4, kRes = RES && ACT != kNone;
+    constexpr bool kExact = sizeof(T) == 4;
     __shared__ float lds[2 * V * 256];
     const Place p = place(g, blockIdx.x);
     float acc[2 * V];                        // sum dz | sum dz (x - mh): the rest of xhat is put in at the end
@@ -341,13 +341,13 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __re
         nc = norm_of<V, S>(g, p, stats);
         const Coef<V, ACT == kRelu> cf = coef_of<V, S, ACT == kRelu>(nc, p.chunk, true, w, b);
         const long col = (long)p.chunk * V, row0 = p.n * g.hw;
-        const T *xb = x + row0 * g.ldx + col, *db = dy + row0 * g.ldd + col, *rb = kRes ? res + row0 * g.ldr + col : nullptr;
+        const T *xb = x + row0 * g.ldx + col, *db = dy + row0 * g.ldd + col, *rb = RES ? res + row0 * g.ldr + col : nullptr;
         Pack<T, V> a[kUnroll], d[kUnroll], e[kUnroll];
         walk(g, p,
              [&](int u, long r) {
                  a[u].load(xb + r * g.ldx);
                  d[u].load(db + r * g.ldd);
-                 if constexpr (kRes) e[u].load(rb + r * g.ldr);
+                 if constexpr (RES) e[u].load(rb + r * g.ldr);
              },
              [&](int u, long) {
 #pragma unroll
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __re
                      float dz = d[u].get(i);
                      if constexpr (ACT != kNone) {
                          float z = cf.z(i, xv, xd);
-                         if constexpr (kRes) z += e[u].get(i);
+                         if constexpr (RES) z += e[u].get(i);
                          dz = act_bwd<ACT, kExact>(dz, z);
                      }
                      acc[i] += dz;
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
                                                            const float* __restrict__ b, const double* __restrict__ stats,
                                                            const float* __restrict__ means, T* __restrict__ dx,
                                                            T* __restrict__ dres) {
-    constexpr bool kExact = sizeof(T) == 4, kRes = RES && ACT != kNone;
+    constexpr bool kExact = sizeof(T) == 4;
     const Place p = place(g, (long)gridDim.x - 1 - blockIdx.x);
     if (!p.on) return;
     const Norm<V, S> nc = norm_of<V, S>(g, p, stats);
@@ -437,14 +437,14 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
         m1[i] = fmaf(-nc.ml[i], k2[i], m[0]);
     }
     const long col = (long)p.chunk * V, row0 = p.n * g.hw;
-    const T *xb = x + row0 * g.ldx + col, *db = dy + row0 * g.ldd + col, *rb = kRes ? res + row0 * g.ldr + col : nullptr;
-    T *ob = dx + row0 * g.C + col, *hb = kRes ? dres + row0 * g.C + col : nullptr;
+    const T *xb = x + row0 * g.ldx + col, *db = dy + row0 * g.ldd + col, *rb = RES ? res + row0 * g.ldr + col : nullptr;
+    T *ob = dx + row0 * g.C + col, *hb = RES ? dres + row0 * g.C + col : nullptr;
     Pack<T, V> a[kUnroll], d[kUnroll], e[kUnroll];
     walk(g, p,
          [&](int u, long r) {
              a[u].load(xb + r * g.ldx);
              d[u].load(db + r * g.ldd);
-             if constexpr (kRes) e[u].load(rb + r * g.ldr);
+             if constexpr (RES) e[u].load(rb + r * g.ldr);
          },
          [&](int u, long r) {
              float f[V], h[V];
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
                  float dz = d[u].get(i);
                  if constexpr (ACT != kNone) {
                      float z = cf.z(i, xv, xd);
-                     if constexpr (kRes) z += e[u].get(i);
+                     if constexpr (RES) z += e[u].get(i);
                      dz = act_bwd<ACT, kExact>(dz, z);
                  }
                  h[i] = dz;
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
                  f[i] = nc.rs[i % S] * fmaf(-xd, k2[i % S], t);
              }
              Pack<T, V>::store(ob + r * g.C, f);
-             if constexpr (kRes) Pack<T, V>::store(hb + r * g.C, h);
+             if constexpr (RES) Pack<T, V>::store(hb + r * g.C, h);
          });
 }
 
@@ -588,7 +588,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
     Pack<T, V> a[K], d[K], e[K];
     slab_load<T, V, K>(a, x, g.ldx, g, s);
     slab_load<T, V, K>(d, dy, g.ldd, g, s);
-    if constexpr (RES && kAct) slab_load<T, V, K>(e, res, g.ldr, g, s);
+    if constexpr (RES) slab_load<T, V, K>(e, res, g.ldr, g, s);
     Norm<V, 1> nc;
     nc.mean[0] = stats[2 * id];
     nc.rstd[0] = stats[2 * id + 1];
@@ -649,7 +649,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
             }
             const long at = (s.n * g.hw + r) * g.C + (long)s.chunk * V;
             Pack<T, V>::store(dx + at, f);
-            if constexpr (RES && kAct) Pack<T, V>::store(dres + at, h);
+            if constexpr (RES) Pack<T, V>::store(dres + at, h);
         }
     }
 }
@@ -787,7 +787,8 @@ template <typename T, int V, int ACT, bool RES> struct RunFwd {
     static int go(const Geo& g, long images, const Fwd& f) { return run_fwd<T, V, ACT, RES>(g, images, f); }
 };
 template <typename T, int V, int ACT, bool RES> struct RunBwd {
-    static int go(const Geo& g, long images, const Bwd& f) { return run_bwd<T, V, ACT, RES>(g, images, f); }
+    // without an activation the residual's gradient is dy and nothing needs the residual
+    static int go(const Geo& g, long images, const Bwd& f) { return run_bwd<T, V, ACT, RES && ACT != kNone>(g, images, f); }
 };
 
 }  // namespace

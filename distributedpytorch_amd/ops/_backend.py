@@ -211,6 +211,12 @@ def launch(what: str, fn, t: torch.Tensor, *args) -> None:
         raise RuntimeError(f"HIP launcher '{what}' failed with status {status}")
 
 
+def first_order(what: str) -> None:
+    """Called by a backward pass whose kernels autograd cannot see into: refuses ``create_graph=True``."""
+    if torch.is_grad_enabled():
+        raise NotImplementedError(f"{what}: no gradients of gradients (create_graph=True)")
+
+
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 

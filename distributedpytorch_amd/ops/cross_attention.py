@@ -18,6 +18,7 @@ from . import _backend as B
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 MAX_DIM = 128
+MAX_LENGTH = 1 << 29
 _sigs = False
 
 
@@ -105,6 +106,7 @@ class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
+        B.first_order("cross_attention")
         q, k, v, out, lse, lens, mask = ctx.saved_tensors
         b, lq, hq, d = q.shape
         meta = (b, lq, k.shape[1], k.shape[2], hq // k.shape[2], d)
@@ -157,6 +159,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     if d > MAX_DIM:
         raise NotImplementedError(f"cross_attention kernels: head widths up to {MAX_DIM}, got {d}; set_backend('torch') "
                                   "runs the plain formulation")
+    if max(b, lq * (hq // hk), lk, hq) > MAX_LENGTH:
+        raise NotImplementedError(f"cross_attention kernels: up to {MAX_LENGTH} images, heads, keys, and positions times the "
+                                  f"query heads of a key head, got q {tuple(q.shape)}, k {tuple(k.shape)}")
     if q.numel() == 0 or lk == 0:
         return (q * 0).nan_to_num(0.0) + (k.sum() + v.sum()) * 0      # zeros, tied to all three inputs
     lens = key_lengths                               # (the kernels limit the values to [0, Lk])

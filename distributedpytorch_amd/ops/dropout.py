@@ -105,6 +105,7 @@ class _Dropout(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        B.first_order("dropout")
         p, seed, use_word = ctx.key
         (held,) = ctx.saved_tensors
         dx = None

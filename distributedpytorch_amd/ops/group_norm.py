@@ -121,6 +121,7 @@ class _GroupNormAct(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        B.first_order("group_norm_act")
         x, residual, w32, b32, stats = ctx.saved_tensors
         groups, act, wdtype, bdtype = ctx.meta
         n, c, h, w = x.shape
@@ -175,6 +176,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
         return group_norm_act_reference(x, num_groups, weight, bias, eps, act, residual)
     if x.dtype not in _DTYPES:
         raise TypeError(f"group_norm_act: bf16, fp16 or fp32 maps, got {x.dtype}")
+    if c > 0x7fffffff:
+        raise NotImplementedError(f"group_norm_act: up to 2^31 - 1 channels, got {c}")
     code = _ACTS[act]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, code)
@@ -212,15 +215,21 @@ class GroupNorm2d(nn.Module):
 
 
 def convert_group_norm(module: nn.Module, num_groups: int = 32) -> nn.Module:
-    """Replace every ``BatchNorm2d`` in ``module`` by a ``GroupNorm2d`` of the same weight and bias (in place), with
-    the largest number of groups that divides both ``num_groups`` and its channels."""
+    """``module`` with every ``BatchNorm2d`` replaced by a ``GroupNorm2d`` of the same weight and bias (in place; a module
+    that is itself one is returned as its replacement), with the largest number of groups that divides both
+    ``num_groups`` and its channels.  A module used in two places stays one module."""
+    return _convert(module, num_groups, {})
+
+
+def _convert(module, num_groups, done):
     from .batchnorm import BatchNorm2d
-    for name, child in module.named_children():
-        if isinstance(child, BatchNorm2d):
-            gn = GroupNorm2d(child.num_features, math.gcd(num_groups, child.num_features), child.eps)
-            gn.weight, gn.bias = child.weight, child.bias
-            gn.train(child.training)
-            setattr(module, name, gn)
-        else:
-            convert_group_norm(child, num_groups)
-    return module
+    if module not in done:
+        done[module] = module
+        if isinstance(module, BatchNorm2d):
+            gn = GroupNorm2d(module.num_features, math.gcd(num_groups, module.num_features), module.eps)
+            gn.weight, gn.bias = module.weight, module.bias
+            done[module] = gn.train(module.training)
+        for name, child in module._modules.items():
+            if child is not None:
+                module._modules[name] = _convert(child, num_groups, done)
+    return done[module]

@@ -109,3 +109,17 @@ def test_variant_checkpoint_round_trip_through_the_predictor(tmp_path):
 def test_variant_refusals(args, kw, err):
     with pytest.raises(err):
         build_model(*args, **kw)
+
+
+def test_convert_group_norm_replaces_the_module_itself_and_shared_ones_once():
+    from distributedpytorch_amd import ops
+    bn = ops.BatchNorm2d(48)
+    gn = ops.convert_group_norm(bn, 32)
+    assert isinstance(gn, ops.GroupNorm2d) and gn.num_groups == 16 and gn.weight is bn.weight and gn.bias is bn.bias
+    shared = ops.BatchNorm2d(8)
+    net = torch.nn.Sequential(shared, torch.nn.Sequential(shared), torch.nn.Identity())
+    net.add_module("again", shared)
+    out = ops.convert_group_norm(net)
+    assert out is net and isinstance(net[0], ops.GroupNorm2d)
+    assert net[0] is net[1][0] and net[0] is net.again
+    assert len(list(net.parameters())) == 2
