@@ -6,6 +6,8 @@
   with ``hipcc --offload-arch=gfx950`` (cross-compiles without a GPU).
 * ``libdpamd_host.so`` — ``host_runtime.cpp``: CPU-side C++ runtime (image warps for the CPU
   transform path, batch collation, bucket planning), compiled with ``g++ -O3 -fopenmp``.
+* ``libdpamd_autograd.so`` — ``autograd.cpp``: autograd nodes and launches of some operators as torch
+  operators (``torch.ops.dpamd``), compiled with ``g++`` against the installed torch.
 
 Staleness is decided by CONTENT, not by mtime (a ``git checkout`` rewrites mtimes arbitrarily): every
 object carries the SHA-256 of its source + the headers + the flags it was built from
@@ -18,6 +20,8 @@ from __future__ import annotations
 import fcntl
 import glob
 import hashlib
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -40,6 +44,8 @@ STRICT_MATH = ("cross_attention.hip", "dropout.hip", "group_norm.hip")
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fopenmp", "-Wall"]
 HIP_LIB = os.path.join(HERE, "libdpamd_hip.so")
 HOST_LIB = os.path.join(HERE, "libdpamd_host.so")
+AUTOGRAD_LIB = os.path.join(HERE, "libdpamd_autograd.so")
+AUTOGRAD_SRC = os.path.join(HERE, "autograd.cpp")
 
 
 def _sha(paths, extra: str = "") -> str:
@@ -73,6 +79,20 @@ def source_hash() -> str:
 
 def host_source_hash() -> str:
     return _sha([os.path.join(HERE, "host_runtime.cpp")] + _headers(), " ".join(HOST_FLAGS))[:32]
+
+
+def autograd_flags():
+    """Flags of ``autograd.cpp``: torch's headers and libraries, found without importing torch."""
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    include = [f"{torch}/include", f"{torch}/include/torch/csrc/api/include",
+               os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
+    return ["-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__", *(f for d in include for f in ("-isystem", d)),
+            f"-L{torch}/lib", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+
+
+def autograd_source_hash() -> str:
+    """Of the source, the flags and torch's version: the library holds that torch's C++ interface."""
+    return _sha([AUTOGRAD_SRC], " ".join([*autograd_flags(), importlib.metadata.version("torch")]))[:32]
 
 
 def _read(path: str) -> str:
@@ -131,6 +151,10 @@ def is_current() -> bool:
     return embedded_hash(HIP_LIB) == source_hash()
 
 
+def autograd_is_current() -> bool:
+    return embedded_hash(AUTOGRAD_LIB, "dp_autograd_build_hash") == autograd_source_hash()
+
+
 def build_all(force: bool = False, verbose: bool = False, save_asm: bool = False) -> bool:
     """Compile whatever is missing or stale; returns True when anything was rebuilt."""
     with _build_lock():
@@ -178,6 +202,15 @@ def _build_all_locked(force: bool, verbose: bool, save_asm: bool) -> bool:
             _run([shutil.which("g++") or "g++", *HOST_FLAGS, "-shared", host_src, stamp_c, "-o", tmp], verbose)
             os.replace(tmp, HOST_LIB)
             rebuilt = True
+    if force or not autograd_is_current():
+        want = autograd_source_hash()
+        stamp_c = os.path.join(OBJ_DIR, "_autograd_stamp.cpp")
+        _write(stamp_c, f'extern "C" const char* dp_autograd_build_hash() {{ return "DP_AUTOGRAD_BUILD_HASH={want}" + 23; }}\n')
+        tmp = AUTOGRAD_LIB + f".{os.getpid()}.tmp"
+        flags = autograd_flags()
+        _run([shutil.which("g++") or "g++", "-shared", AUTOGRAD_SRC, stamp_c, "-o", tmp, *flags], verbose)
+        os.replace(tmp, AUTOGRAD_LIB)
+        rebuilt = True
     return rebuilt
 
 
@@ -201,8 +234,8 @@ if __name__ == "__main__":
         print("built:", build_host_sanitized(verbose=True))
         sys.exit(0)
     if "--check" in sys.argv:
-        ok = is_current()
-        print("libdpamd_hip.so", "is current" if ok else "is STALE or missing", source_hash())
+        ok = is_current() and autograd_is_current()
+        print("libdpamd_hip.so, libdpamd_autograd.so", "are current" if ok else "are STALE or missing", source_hash())
         sys.exit(0 if ok else 1)
     build_all(force="--force" in sys.argv, verbose=True, save_asm="--asm" in sys.argv)
     print("built:", [f for f in os.listdir(HERE) if f.endswith(".so")], "hash", source_hash())

@@ -27,6 +27,7 @@ HOST_LIB_PATH = os.path.join(os.path.dirname(_HERE), "csrc", "libdpamd_host.so")
 _lock = threading.Lock()
 _lib = None
 _host_lib = None
+_native = None
 _mode = os.environ.get("DPAMD_BACKEND", "auto")  # 'auto' | 'torch'
 
 
@@ -172,6 +173,31 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+# the launchers that libdpamd_autograd.so calls, in the order of its table
+_BOUND = ("dp_gn_workspace", "dp_gn_fwd", "dp_gn_bwd", "dp_dropout", "dp_xa_workspace", "dp_xa_fwd", "dp_xa_bwd")
+
+
+def native():
+    """``torch.ops.dpamd``: operators whose autograd nodes and launches are C++ (csrc/autograd.cpp).  Built and loaded as
+    ``lib()`` is, whose launchers it calls."""
+    global _native
+    if _native is None:
+        kernels = lib()
+        with _lock:
+            if _native is None:
+                from ..csrc import build as _b
+                if not _b.autograd_is_current():
+                    if os.environ.get("DPAMD_AUTO_BUILD", "1") == "0":
+                        raise NativeLibraryMissing(f"{_b.AUTOGRAD_LIB} missing or stale: run "
+                                                   "`python -m distributedpytorch_amd.csrc.build`")
+                    print(f"[dpamd] {_b.AUTOGRAD_LIB} missing or stale: building in-tree ...", file=sys.stderr, flush=True)
+                    _b.build_all(verbose=False)
+                torch.ops.load_library(_b.AUTOGRAD_LIB)
+                torch.ops.dpamd.bind([ctypes.cast(getattr(kernels, f), ctypes.c_void_p).value for f in _BOUND])
+                _native = torch.ops.dpamd
+    return _native
+
+
 def host_lib() -> ctypes.CDLL | None:
     """The host-side C++ runtime (CPU image warps, bucket planner).  Optional on CPU."""
     global _host_lib
@@ -194,27 +220,6 @@ def lib_current() -> bool:
 def stream_ptr() -> ctypes.c_void_p:
     """Current HIP stream as a raw ``hipStream_t`` for the C launchers."""
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-def launch(what: str, fn, t: torch.Tensor, *args) -> None:
-    """``fn(*args, stream)`` on the GPU of ``t`` and its current stream, whichever GPU is current; raises on a status.
-
-    Few Python steps on purpose: a backward pass runs in autograd's own thread, where every Python object that the
-    forward thread touched last is a cache miss (finding the stream through ``torch.cuda`` took 18 us there)."""
-    index = t.get_device()
-    if index == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status != 0:
-        raise RuntimeError(f"HIP launcher '{what}' failed with status {status}")
-
-
-def first_order(what: str) -> None:
-    """Called by a backward pass whose kernels autograd cannot see into: refuses ``create_graph=True``."""
-    if torch.is_grad_enabled():
-        raise NotImplementedError(f"{what}: no gradients of gradients (create_graph=True)")
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

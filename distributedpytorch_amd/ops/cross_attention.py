@@ -1,4 +1,5 @@
-"""Attention of one sequence's queries over another's keys and values (csrc/cross_attention.hip).
+"""Attention of one sequence's queries over another's keys and values (csrc/cross_attention.hip,
+csrc/autograd.cpp).
 
 ``position_attention`` (ops.attention) is DANet's: one head, every position of a map over the same map, no mask.  Here the
 two lengths differ, heads are split and may share keys, and images may hold fewer keys than the tensor has room for — a
@@ -7,8 +8,6 @@ plain torch operations.
 """
 from __future__ import annotations
 
-import ctypes
-import functools
 import math
 from typing import Optional
 
@@ -16,23 +15,9 @@ import torch
 
 from . import _backend as B
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_TYPES = (torch.bfloat16, torch.float16)
 MAX_DIM = 128
 MAX_LENGTH = 1 << 29
-_sigs = False
-
-
-def _lib():
-    global _sigs
-    lib = B.lib()
-    if not _sigs:
-        V, L, I, F = ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_float
-        lib.dp_xa_workspace.argtypes = [I] * 7
-        lib.dp_xa_workspace.restype = L
-        lib.dp_xa_fwd.argtypes = [V] * 7 + [L, V, V] + [I] * 6 + [F, I, V]
-        lib.dp_xa_bwd.argtypes = [V] * 12 + [L, V, V] + [I] * 6 + [F, I, V]
-        _sigs = True
-    return lib
 
 
 def cross_attention_reference(q, k, v, key_lengths=None, key_mask=None, scale=None):
@@ -55,69 +40,6 @@ def cross_attention_reference(q, k, v, key_lengths=None, key_mask=None, scale=No
     p = torch.softmax(torch.where(some, s, zero), dim=-1) if lk else s
     o = torch.matmul(torch.where(some, p, zero), vf.contiguous())
     return o.permute(0, 2, 1, 3).contiguous().to(q.dtype)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` where the kernels can read its rows as 16-byte pieces, a dense copy otherwise."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s >= 0 and s % 8 == 0)
-                                                            for n, s in zip(t.shape[:3], t.stride()[:3]))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
-
-
-def _strides(*ts):
-    flat = [0 if n == 1 else s for t in ts for n, s in zip(t.shape[:3], t.stride()[:3])]
-    return (ctypes.c_long * len(flat))(*flat)
-
-
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-@functools.lru_cache(maxsize=4096)
-def _workspace_floats(meta, backward) -> int:
-    return int(_lib().dp_xa_workspace(*meta, backward))
-
-
-def _workspace(meta, q, backward):
-    need = _workspace_floats(meta, backward)
-    return torch.empty(need, dtype=torch.float32, device=q.device) if need > 0 else None
-
-
-def _forward(q, k, v, lens, mask, scale, need_lse):
-    b, lq, hq, d = q.shape
-    lk, hk = k.shape[1], k.shape[2]
-    meta = (b, lq, lk, hk, hq // hk, d)
-    out = torch.empty((b, lq, hq, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, hk, lq * (hq // hk)), dtype=torch.float32, device=q.device) if need_lse else None
-    ws = _workspace(meta, q, 0)
-    B.launch("xa_fwd", _lib().dp_xa_fwd, q, _p(q), _p(k), _p(v), _p(out), _p(lse), _p(lens), _p(mask),
-             0 if mask is None else mask.stride(0), _p(ws), _strides(q, k, v), *meta, scale, _DTYPES[q.dtype])
-    return out, lse
-
-
-class _CrossAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, lens, mask, scale):
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        out, lse = _forward(q, k, v, lens, mask, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, lens, mask)
-        ctx.scale = scale
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        B.first_order("cross_attention")
-        q, k, v, out, lse, lens, mask = ctx.saved_tensors
-        b, lq, hq, d = q.shape
-        meta = (b, lq, k.shape[1], k.shape[2], hq // k.shape[2], d)
-        dout = _rows(dout)
-        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-        delta = torch.empty_like(lse)
-        ws = _workspace(meta, q, 1)
-        B.launch("xa_bwd", _lib().dp_xa_bwd, q, _p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(delta), _p(dq), _p(dk),
-                 _p(dv), _p(lens), _p(mask), 0 if mask is None else mask.stride(0), _p(ws), _strides(q, k, v, dout), *meta,
-                 ctx.scale, _DTYPES[q.dtype])
-        return dq, dk, dv, None, None, None
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengths: Optional[torch.Tensor] = None,
@@ -154,7 +76,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
                              f"{tuple(key_mask.shape)} {key_mask.dtype} on {key_mask.device}")
     if not B.use_hip(q):
         return cross_attention_reference(q, k, v, key_lengths, key_mask, scale)
-    if q.dtype not in _DTYPES:
+    if q.dtype not in _TYPES:
         raise TypeError(f"cross_attention kernels: bf16 or fp16, got {q.dtype}; set_backend('torch') runs the plain formulation")
     if d > MAX_DIM:
         raise NotImplementedError(f"cross_attention kernels: head widths up to {MAX_DIM}, got {d}; set_backend('torch') "
@@ -171,8 +93,5 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     if d % 8:
         # zero columns are exact: they add nothing to q kᵀ, and zero value columns are sliced off again
         q, k, v = (torch.nn.functional.pad(t, (0, 8 - d % 8)) for t in (q, k, v))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out = _CrossAttention.apply(q, k, v, lens, mask, scale)
-    else:
-        out = _forward(_rows(q), _rows(k), _rows(v), lens, mask, scale, False)[0]
+    out = B.native().cross_attention.default(q, k, v, lens, mask, scale)
     return out[..., :d] if d % 8 else out

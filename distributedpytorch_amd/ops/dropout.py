@@ -1,4 +1,4 @@
-"""Dropout whose mask is a function of (seed, position) and is never stored (csrc/dropout.hip).
+"""Dropout whose mask is a function of (seed, position) and is never stored (csrc/dropout.hip, csrc/autograd.cpp).
 
 The keep decision of an element comes from Philox4x32-10 (Salmon et al. 2011) under a 64-bit seed: block ``j`` of eight
 elements in memory order has the counter ``(j, j >> 32, 0, 0)``, each 32-bit word decides two elements, and backward
@@ -7,7 +7,6 @@ operations: one seed gives one mask everywhere.
 """
 from __future__ import annotations
 
-import ctypes
 import operator
 from typing import Optional, Union
 
@@ -15,19 +14,8 @@ import torch
 
 from . import _backend as B
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _LOW = 0xFFFFFFFF
-_sigs = False
-
-
-def _lib():
-    global _sigs
-    lib = B.lib()
-    if not _sigs:
-        V, L, I = ctypes.c_void_p, ctypes.c_long, ctypes.c_int
-        lib.dp_dropout.argtypes = [V, V, V, L, ctypes.c_uint, ctypes.c_ulonglong, V, I, I, V]
-        _sigs = True
-    return lib
 
 
 def dropout_threshold(p: float) -> int:
@@ -71,50 +59,39 @@ def _memory_order(t: torch.Tensor) -> torch.Tensor:
     return t.as_strided((t.numel(),), (1,))
 
 
-def _run(x, residual, p, seed, use_word):
+def _run(x, residual, p, seed):
     """``x`` dense; ``residual`` in the same order or None."""
-    if not B.use_hip(x):
-        keep = dropout_keep(x.numel(), seed, p, x.device)
-        wide = x if x.dtype == torch.float64 else x.float()
-        thr = dropout_threshold(p)
-        flat = torch.where(keep, _memory_order(wide) * (65536.0 / (65536.0 - thr) if thr < 65536 else 0.0),
-                           torch.zeros((), dtype=wide.dtype, device=x.device))
-        if residual is not None:
-            flat = flat + _memory_order(residual).to(flat.dtype)
-        out = torch.empty_like(x)
-        _memory_order(out).copy_(flat)
-        return out
-    y = torch.empty_like(x)
-    if x.numel() == 0:
-        return y
-    dev = isinstance(seed, torch.Tensor)
-    B.launch("dropout", _lib().dp_dropout, x, x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(),
-             x.numel(), dropout_threshold(p), 0 if dev else seed, seed.data_ptr() if dev else None, use_word,
-             _DTYPES[x.dtype])
-    return y
+    keep = dropout_keep(x.numel(), seed, p, x.device)
+    wide = x if x.dtype == torch.float64 else x.float()
+    thr = dropout_threshold(p)
+    flat = torch.where(keep, _memory_order(wide) * (65536.0 / (65536.0 - thr) if thr < 65536 else 0.0),
+                       torch.zeros((), dtype=wide.dtype, device=x.device))
+    if residual is not None:
+        flat = flat + _memory_order(residual).to(flat.dtype)
+    out = torch.empty_like(x)
+    _memory_order(out).copy_(flat)
+    return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, use_word):
+    def forward(ctx, x, residual, p, seed):
         x = _dense(x)
-        ctx.key = (p, None if isinstance(seed, torch.Tensor) else seed, use_word)
+        ctx.p, ctx.seed, ctx.strides = p, None if isinstance(seed, torch.Tensor) else seed, x.stride()
         ctx.save_for_backward(seed if isinstance(seed, torch.Tensor) else None)
-        ctx.strides = x.stride()
-        return _run(x, None if residual is None else _like(residual, x), p, seed, use_word)
+        return _run(x, None if residual is None else _like(residual, x), p, seed)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        B.first_order("dropout")
-        p, seed, use_word = ctx.key
         (held,) = ctx.saved_tensors
         dx = None
         if ctx.needs_input_grad[0]:
             g = dy
             if g.stride() != ctx.strides:          # the mask follows the memory order of the forward's input
                 g = torch.empty_strided(dy.shape, ctx.strides, dtype=dy.dtype, device=dy.device).copy_(dy)
-            dx = _run(g, None, p, held if held is not None else seed, use_word)
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+            dx = _run(g, None, ctx.p, held if held is not None else ctx.seed)
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None
 
 
 def dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, seed: Optional[Union[int, torch.Tensor]] = None,
@@ -139,7 +116,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, seed: Option
         seed = seed.reshape(1)
     if not training or p == 0.0:
         return x if residual is None else x + residual
-    if not x.is_floating_point() or (B.use_hip(x) and x.dtype not in _DTYPES):
+    if not x.is_floating_point() or (B.use_hip(x) and x.dtype not in _TYPES):
         raise TypeError(f"dropout: bf16, fp16 or fp32 tensors, got {x.dtype}")
     use_word = seed is None
     if use_word:
@@ -147,7 +124,11 @@ def dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, seed: Option
         seed = _dropout_key(p)[1]
     elif not isinstance(seed, torch.Tensor):
         seed = operator.index(seed) & 0xFFFFFFFFFFFFFFFF
+    if B.use_hip(x):
+        held = isinstance(seed, torch.Tensor)
+        number = 0 if held else seed - (1 << 64) if seed >= 1 << 63 else seed            # (as a signed 64-bit number)
+        return B.native().dropout.default(x, residual, dropout_threshold(p), number, seed if held else None, use_word)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, p, seed, use_word)
+        return _Dropout.apply(x, residual, p, seed)
     x = _dense(x)
-    return _run(x, None if residual is None else _like(residual, x), p, seed, use_word)
+    return _run(x, None if residual is None else _like(residual, x), p, seed)

@@ -1,4 +1,4 @@
-"""Group normalisation of channels-last maps fused with a residual and an activation (csrc/group_norm.hip).
+"""Group normalisation of channels-last maps fused with a residual and an activation (csrc/group_norm.hip, csrc/autograd.cpp).
 
 The counterpart of ``batch_norm_act`` whose statistics come from one image's group of channels: nothing depends on the
 batch, so it serves training at a few images per GPU, and evaluation computes what training computes.  CPU tensors /
@@ -6,8 +6,6 @@ batch, so it serves training at a few images per GPU, and evaluation computes wh
 """
 from __future__ import annotations
 
-import ctypes
-import functools
 import math
 from typing import Optional
 
@@ -15,24 +13,9 @@ import torch
 import torch.nn as nn
 
 from . import _backend as B
-from .concat import row_stride
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2}
-_sigs = False
-
-
-def _lib():
-    global _sigs
-    lib = B.lib()
-    if not _sigs:
-        V, L, I, F = ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_float
-        lib.dp_gn_workspace.argtypes = [L, L, I, I, I]
-        lib.dp_gn_workspace.restype = L
-        lib.dp_gn_fwd.argtypes = [V] * 7 + [L, L, I, I, L, L, F, I, I, V]
-        lib.dp_gn_bwd.argtypes = [V] * 11 + [L, L, I, I, L, L, L, I, I, V]
-        _sigs = True
-    return lib
 
 
 def group_norm_act_reference(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, residual=None):
@@ -55,100 +38,6 @@ def group_norm_act_reference(x, num_groups, weight=None, bias=None, eps=1e-5, ac
     elif _ACTS[act] == 2:
         z = z * torch.sigmoid(z)
     return z.to(x.dtype)
-
-
-def _rows(t: torch.Tensor):
-    """(tensor, elements between rows): ``t`` as it is when its memory is NHWC rows (a channels-last map or a channel
-    slice of one), a channels-last copy otherwise."""
-    ld = t.shape[1]
-    if t.is_contiguous(memory_format=torch.channels_last):
-        return t, ld
-    ld = row_stride(t)
-    if ld is None:
-        t = t.contiguous(memory_format=torch.channels_last)
-        ld = t.shape[1]
-    return t, ld
-
-
-def _p(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _vec(t: Optional[torch.Tensor]):
-    if t is None:
-        return None
-    t = t.detach()
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
-
-
-def _new(x: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(x, memory_format=torch.channels_last)
-
-
-@functools.lru_cache(maxsize=4096)
-def _workspace_floats(n, hw, c, groups, esize) -> int:
-    return int(_lib().dp_gn_workspace(n, hw, c, groups, esize))
-
-
-def _workspace(x, n, hw, c, groups):
-    return torch.empty(_workspace_floats(n, hw, c, groups, x.element_size()), dtype=torch.float32, device=x.device)
-
-
-def _forward(x, groups, weight, bias, eps, act, residual):
-    n, c, h, w = x.shape
-    y = _new(x)
-    stats = torch.empty((n, groups, 2), dtype=torch.float64, device=x.device)
-    if x.numel():
-        x, ldx = _rows(x)
-        ldr = c
-        if residual is not None:
-            residual, ldr = _rows(residual)
-        ws = _workspace(x, n, h * w, c, groups)
-        B.launch("gn_fwd", _lib().dp_gn_fwd, x, _p(x), _p(residual), _p(weight), _p(bias), _p(y), _p(stats), _p(ws), n, h * w,
-                 c, groups, ldx, ldr, eps, act, _DTYPES[x.dtype])
-    return y, stats
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, groups, eps, act):
-        w32, b32 = _vec(weight), _vec(bias)
-        y, stats = _forward(x, groups, w32, b32, eps, act, residual)
-        # an activation's derivative needs z: the residual is kept for it (without one its gradient is dy itself)
-        ctx.save_for_backward(x, residual if act else None, w32, b32, stats)
-        ctx.meta = (groups, act, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        B.first_order("group_norm_act")
-        x, residual, w32, b32, stats = ctx.saved_tensors
-        groups, act, wdtype, bdtype = ctx.meta
-        n, c, h, w = x.shape
-        dx = _new(x)
-        dres = _new(x) if residual is not None else None
-        dw = None if wdtype is None else torch.empty_like(w32)
-        db = None if bdtype is None else torch.empty_like(b32)
-        if x.numel():
-            x, ldx = _rows(x)
-            g, ldd = _rows(dy)
-            ldr = c
-            if residual is not None:
-                residual, ldr = _rows(residual)
-            ws = _workspace(x, n, h * w, c, groups)
-            B.launch("gn_bwd", _lib().dp_gn_bwd, x, _p(g), _p(x), _p(residual), _p(w32), _p(b32), _p(stats), _p(dx), _p(dres),
-                     _p(dw), _p(db), _p(ws), n, h * w, c, groups, ldx, ldr, ldd, act, _DTYPES[x.dtype])
-        else:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        if dres is None and ctx.needs_input_grad[3]:
-            dres = dy                                     # no activation: the residual's gradient is dy
-        if dw is not None and wdtype != torch.float32:
-            dw = dw.to(wdtype)
-        if db is not None and bdtype != torch.float32:
-            db = db.to(bdtype)
-        return dx, dw, db, dres, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
@@ -174,14 +63,11 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
                          f"match x {tuple(x.shape)} {x.dtype} {x.device}")
     if not B.use_hip(x):
         return group_norm_act_reference(x, num_groups, weight, bias, eps, act, residual)
-    if x.dtype not in _DTYPES:
+    if x.dtype not in _TYPES:
         raise TypeError(f"group_norm_act: bf16, fp16 or fp32 maps, got {x.dtype}")
     if c > 0x7fffffff:
         raise NotImplementedError(f"group_norm_act: up to 2^31 - 1 channels, got {c}")
-    code = _ACTS[act]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, code)
-    return _forward(x, num_groups, _vec(weight), _vec(bias), eps, code, residual)[0]
+    return B.native().group_norm_act.default(x, weight, bias, residual, num_groups, eps, _ACTS[act])
 
 
 class GroupNorm2d(nn.Module):
