@@ -167,15 +167,15 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     return v;
 }
 
-// A team of `wide` waves (1 or 4, whole in one block of 256 threads) takes one (image, group): its items are the group's
+// A team of `wide` waves (1 or 4, whole in one block of N threads) takes one (image, group): its items are the group's
 // (row range, channel) pairs, in memory order.
 struct Team { long gi, n; int c0, items, first, step; bool on; };
 
-__device__ __forceinline__ Team team_of(const Geo& g, long groups, int wide, long block) {
+template <int N> __device__ __forceinline__ Team team_of(const Geo& g, long groups, int wide, long block) {
     const int tid = threadIdx.x;
     Team t;
     t.step = wide * 64;
-    t.gi = block * (4 / wide) + tid / t.step;
+    t.gi = block * (N / 64 / wide) + tid / t.step;
     t.on = t.gi < groups;
     t.n = t.on ? t.gi / g.G : 0;
     t.c0 = t.on ? (int)(t.gi % g.G) * g.cpg : 0;
@@ -191,7 +191,8 @@ __device__ __forceinline__ double team_sum(double v, int wide, double* lds) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[w] = v;
     __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    const double* own = lds + (w & ~3);
+    return (own[0] + own[1]) + (own[2] + own[3]);
 }
 
 // stats[n, g] = (mean, rstd).  Every item is a sample with a mean and squared deviations of its own; all the terms that
@@ -199,7 +200,7 @@ __device__ __forceinline__ double team_sum(double v, int wide, double* lds) {
 __global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int wide, const float* __restrict__ part,
                                                         const float* __restrict__ pivot, double* __restrict__ stats) {
     __shared__ double lds[4];
-    const Team t = team_of(g, groups, wide, blockIdx.x);
+    const Team t = team_of<256>(g, groups, wide, blockIdx.x);
     const float* base = part + t.n * g.splits * 2 * g.C + t.c0;
     const float* pv = pivot + t.n * g.C + t.c0;
     double sm = 0.0;
@@ -372,45 +373,51 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __re
     }
 }
 
-// means[n, g] = (m1, m2)
-__global__ __launch_bounds__(256) void gn_bwd_means_kernel(Geo g, long groups, int wide, const float* __restrict__ part,
-                                                           const float* __restrict__ w, float* __restrict__ means) {
-    __shared__ double lds[4];
-    const Team t = team_of(g, groups, wide, blockIdx.x);
-    const float* base = part + t.n * g.splits * 2 * g.C + t.c0;
-    double a = 0.0, q = 0.0;
-#pragma unroll 4
-    for (int i = t.first; i < t.items; i += t.step) {
-        const int s = i / g.cpg, c = i - s * g.cpg;
-        const double wc = w ? (double)w[t.c0 + c] : 1.0;
-        a += wc * (double)base[(long)s * 2 * g.C + c];
-        q += wc * (double)base[(long)s * 2 * g.C + g.C + c];
-    }
-    a = team_sum(a, wide, lds);
-    q = team_sum(q, wide, lds);
-    if (t.on && t.first == 0) {
-        const double inv = 1.0 / ((double)g.hw * g.cpg);
-        means[2 * t.gi] = (float)(a * inv);
-        means[2 * t.gi + 1] = (float)(q * inv);
-    }
-}
+// The first mean_blocks blocks: means[n, g] = (m1, m2), a team a group.  The others: dw and db, 16 channels by 64 lines of
+// parts a block.
+constexpr int kJoin = 1024;
 
-// dw and db: 16 channels by 64 lines of parts a block
-__global__ __launch_bounds__(1024) void gn_bwd_params_kernel(int C, long lines, const float* __restrict__ part,
-                                                             float* __restrict__ dw, float* __restrict__ db) {
-    __shared__ double lds[2][1024];
-    const int tid = threadIdx.x, c = blockIdx.x * 16 + (tid & 15);
+__global__ __launch_bounds__(kJoin) void gn_bwd_join_kernel(Geo g, long groups, int wide, int mean_blocks, long lines,
+                                                            const float* __restrict__ part, const float* __restrict__ w,
+                                                            float* __restrict__ means, float* __restrict__ dw,
+                                                            float* __restrict__ db) {
+    __shared__ double lds[2][kJoin];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < mean_blocks) {
+        const Team t = team_of<kJoin>(g, groups, wide, blockIdx.x);
+        const float* base = part + t.n * g.splits * 2 * g.C + t.c0;
+        double a = 0.0, q = 0.0;
+#pragma unroll 4
+        for (int i = t.first; i < t.items; i += t.step) {
+            const int s = i / g.cpg, c = i - s * g.cpg;
+            const double wc = w ? (double)w[t.c0 + c] : 1.0;
+            a += wc * (double)base[(long)s * 2 * g.C + c];
+            q += wc * (double)base[(long)s * 2 * g.C + g.C + c];
+        }
+        a = team_sum(a, wide, lds[0]);
+        q = team_sum(q, wide, lds[1]);
+        if (t.on && t.first == 0) {
+            const double inv = 1.0 / ((double)g.hw * g.cpg);
+            means[2 * t.gi] = (float)(a * inv);
+            means[2 * t.gi + 1] = (float)(q * inv);
+        }
+        return;
+    }
+    const int c = ((int)blockIdx.x - mean_blocks) * 16 + (tid & 15);
     double s1 = 0.0, s2 = 0.0;
-    if (c < C)
+    if (c < g.C)
 #pragma unroll 8
-        for (long k = tid >> 4; k < lines; k += 64) { s1 += (double)part[2 * k * C + c]; s2 += (double)part[(2 * k + 1) * C + c]; }
+        for (long k = tid >> 4; k < lines; k += kJoin / 16) {
+            s1 += (double)part[2 * k * g.C + c];
+            s2 += (double)part[(2 * k + 1) * g.C + c];
+        }
     lds[0][tid] = s1;
     lds[1][tid] = s2;
-    for (int s = 512; s >= 16; s >>= 1) {
+    for (int s = kJoin / 2; s >= 16; s >>= 1) {
         __syncthreads();
         if (tid < s) { lds[0][tid] += lds[0][tid + s]; lds[1][tid] += lds[1][tid + s]; }
     }
-    if (tid < 16 && c < C) {
+    if (tid < 16 && c < g.C) {
         if (dw) dw[c] = (float)lds[1][tid];
         if (db) db[c] = (float)lds[0][tid];
     }
@@ -686,7 +693,8 @@ Geo make_geo(long images, long hw, int C, int G, int V, float eps, long ldx, lon
 // waves of a team: four where a group has more than a wave's worth of items
 int team_width(const Geo& g) { return (long)g.cpg * g.splits > 64 ? 4 : 1; }
 
-dim3 team_grid(long groups, int wide) { return dim3((unsigned)(wide == 4 ? groups : (groups + 3) / 4)); }
+// blocks of `waves` waves for all teams
+long team_blocks(long groups, int wide, int waves) { return (groups * wide + waves - 1) / waves; }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -723,7 +731,7 @@ int run_fwd(const Geo& g, long images, const Fwd& f) {
     float* pivot = f.ws;
     float* part = f.ws + images * g.C;
     gn_stats_kernel<T, V><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, part, pivot);
-    gn_finish_kernel<<<team_grid(groups, wide), 256, 0, f.stream>>>(g, groups, wide, part, pivot, f.stats);
+    gn_finish_kernel<<<dim3((unsigned)team_blocks(groups, wide, 4)), 256, 0, f.stream>>>(g, groups, wide, part, pivot, f.stats);
     const auto apply = g.cpg % V == 0 ? gn_apply_kernel<T, V, 1, ACT, RES> : gn_apply_kernel<T, V, V, ACT, RES>;
     apply<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, (T*)f.y);
     return DP_LAUNCH_STATUS();
@@ -738,13 +746,13 @@ template <typename T, int V, int ACT, bool RES>
 int run_bwd(const Geo& g, long images, const Bwd& f) {
     const long blocks = images * g.cblocks * g.splits, groups = images * g.G;
     const int wide = team_width(g);
+    const unsigned sums = f.dw || f.db ? (unsigned)(((long)g.C + 15) / 16) : 0;
     if (blocks > 0x7fffffffL || groups > 0x7fffffffL) return -3;
     if constexpr (V > 1) {
         if (fits_slab(g, V, RES)) {
             gn_slab_bwd_kernel<T, V, ACT, RES><<<dim3((unsigned)groups), kBlock, 0, f.stream>>>(
                 make_slab(g, V), (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, (T*)f.dx, (T*)f.dres, f.ws);
-            if (f.dw || f.db)
-                gn_bwd_params_kernel<<<dim3((unsigned)((g.C + 15) / 16)), 1024, 0, f.stream>>>(g.C, images, f.ws, f.dw, f.db);
+            if (sums) gn_bwd_join_kernel<<<dim3(sums), kJoin, 0, f.stream>>>(g, 0, 1, 0, images, f.ws, f.w, nullptr, f.dw, f.db);
             return DP_LAUNCH_STATUS();
         }
     }
@@ -755,9 +763,9 @@ int run_bwd(const Geo& g, long images, const Bwd& f) {
     const auto apply = one ? gn_bwd_apply_kernel<T, V, 1, ACT, RES> : gn_bwd_apply_kernel<T, V, V, ACT, RES>;
     reduce<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, part);
-    gn_bwd_means_kernel<<<team_grid(groups, wide), 256, 0, f.stream>>>(g, groups, wide, part, f.w, means);
-    if (f.dw || f.db)
-        gn_bwd_params_kernel<<<dim3((unsigned)((g.C + 15) / 16)), 1024, 0, f.stream>>>(g.C, images * g.splits, part, f.dw, f.db);
+    const unsigned mean_blocks = (unsigned)team_blocks(groups, wide, kJoin / 64);
+    gn_bwd_join_kernel<<<dim3(mean_blocks + sums), kJoin, 0, f.stream>>>(g, groups, wide, (int)mean_blocks, images * g.splits,
+                                                                        part, f.w, means, f.dw, f.db);
     apply<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, means, (T*)f.dx, (T*)f.dres);
     return DP_LAUNCH_STATUS();
