@@ -144,6 +144,14 @@ template <typename E> __device__ __forceinline__ uint4 pack_acc(const f32x16& a,
 // entry of the 32 that accumulator register r of lane half h belongs to
 __device__ __forceinline__ int entry(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
+// Whether the key of accumulator register i of 32-key tile t takes part, for this lane.  The set is a scalar: its two bits (of
+// the lane halves) become a lane mask on the scalar unit, and the select is all that the vector unit does.
+__device__ __forceinline__ bool key_on(unsigned long long set, int t, int i) {
+    const unsigned bits = (unsigned)(set >> (32 * t));
+    const unsigned lo = (unsigned)((int)(bits << (31 - entry(i, 0))) >> 31), hi = (unsigned)((int)(bits << (31 - entry(i, 1))) >> 31);
+    return __builtin_amdgcn_inverse_ballot_w64((unsigned long long)hi << 32 | lo);
+}
+
 __device__ __forceinline__ float row_max(const f32x16 (&s)[2]) {
     float mx = s[0][0];
 #pragma unroll
@@ -360,6 +368,10 @@ __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
     return w;
 }
 
+// Where part s of `blocks` begins (at most 2^23 blocks and 64 parts: the product fits 32 bits, whose division is a tenth of
+// a 64-bit one's instructions).
+__device__ __forceinline__ int part_of(int blocks, int s, int parts) { return (int)((unsigned)blocks * (unsigned)s / (unsigned)parts); }
+
 // ------------------------------------------------------------------------------------------------ forward
 template <typename E, int DP, bool DMA>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, int tiles) {
@@ -373,7 +385,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, in
     const bool row_on = r < p.R, wave_on = r - l31 < p.R;
     const int len = key_count(p, w.b);
     const int nkb = (len + kKeys - 1) / kKeys;
-    const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
+    const int kb0 = part_of(nkb, w.split, p.splits), kb1 = part_of(nkb, w.split + 1, p.splits);
 
     uint4 qf[DP / 16];
     row_operand<T, DP>(p, p.q, p.vq, w.b, w.hk, r, row_on, qf);
@@ -416,11 +428,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, in
         float top = row_max(st);
         if (set != ~0ull) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) st[t][i] = (bits >> entry(i, 0) & 1) ? st[t][i] : -kInf;
-            }
+                for (int i = 0; i < 16; ++i) st[t][i] = key_on(set, t, i) ? st[t][i] : -kInf;
             top = row_max(st);
         }
         top = halves_max(top);
@@ -492,14 +502,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, in
 // joins the splits of one row: a wave per row, its parts' statistics in one access and its sums in the next: 6.6 us for 64
 // rows of 17 parts, 21 us for 33,800 rows of 5 parts of 128 columns (88 MB: 4.2 TB/s)
 template <typename E, int DP>
-__global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
+__global__ __launch_bounds__(256) void xa_join_kernel(Att p, unsigned rows) {
     typedef typename E::raw T;
-    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const unsigned id = blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (id >= rows) return;
-    const long bh = id / p.R;
-    const int r = (int)(id - bh * p.R);
-    const float* base = p.part + (bh * p.splits * p.R + r) * (DP + 2);
+    const unsigned bh = id / (unsigned)p.R, r = id - bh * (unsigned)p.R;
+    const float* base = p.part + ((long)bh * p.splits * p.R + r) * (DP + 2);
     const long step = (long)p.R * (DP + 2);
     // lane s weighs part s (at most 64 parts)
     const float own = lane < p.splits ? base[lane * step + DP] : -kInf, sum = lane < p.splits ? base[lane * step + DP + 1] : 0.f;
@@ -522,8 +531,7 @@ __global__ __launch_bounds__(256) void xa_join_kernel(Att p, long rows) {
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     if (lane == 0 && p.lse) p.lse[id] = log_sum(m, l, p.c);
     if (d < p.D) {
-        const int b = (int)(bh / p.Hk), hk = (int)(bh % p.Hk);
-        T* o = (T*)p.out + dense_row(p, b, hk, r);
+        T* o = (T*)p.out + dense_row(p, bh / (unsigned)p.Hk, bh % (unsigned)p.Hk, r);
         *reinterpret_cast<unsigned*>(o + d) = E::pair(a0 * inv, a1 * inv);
     }
 }
@@ -543,7 +551,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
     const bool row_on = r < p.R, wave_on = w.tile * kRows + wave * 32 < p.R;
     const int len = key_count(p, w.b);
     const int nkb = (len + kKeys - 1) / kKeys;
-    const int kb0 = (int)((long)nkb * w.split / p.splits), kb1 = (int)((long)nkb * (w.split + 1) / p.splits);
+    const int kb0 = part_of(nkb, w.split, p.splits), kb1 = part_of(nkb, w.split + 1, p.splits);
     const long bh = (long)w.b * p.Hk + w.hk;
 
     uint4 qf[DP / 16], df[DP / 16];
@@ -610,9 +618,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse)) * dp[i];
             if (set != ~0ull) {
-                const unsigned bits = (unsigned)(set >> (32 * t)) >> (4 * h);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = (bits >> entry(i, 0) & 1) ? s[i] : 0.f;
+                for (int i = 0; i < 16; ++i) s[i] = key_on(set, t, i) ? s[i] : 0.f;
             }
         };
         if (nkb == 1) {
@@ -668,7 +675,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
 // dk and dv of 128 keys.  A key is a column of every product here, so what a masked key's lane computes reaches no other:
 // it is thrown away at the end.
 template <typename E, int DP, bool DMA>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, int tiles) {
+__global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void xa_dkv_kernel(Att p, int tiles) {
     typedef typename E::raw T;
     __shared__ __attribute__((aligned(16))) unsigned char Q0[Tile<DP>::kBytes], D0[Tile<DP>::kBytes], Q1[Tile<DP>::kBytes],
         D1[Tile<DP>::kBytes];
@@ -682,8 +689,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
     const bool wave_on = __any(on);
     const long bh = (long)w.b * p.Hk + w.hk;
     const int nst = (p.R + kStep - 1) / kStep;
-    const int st0 = (int)((long)nst * w.split / p.splits);
-    const int st1 = w.tile * kRows < len ? (int)((long)nst * (w.split + 1) / p.splits) : st0;
+    const int st0 = part_of(nst, w.split, p.splits);
+    const int st1 = w.tile * kRows < len ? part_of(nst, w.split + 1, p.splits) : st0;
 
     uint4 kf[DP / 16], vf[DP / 16];
 #pragma unroll
@@ -804,21 +811,26 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void xa_dkv_kernel(Att p, in
         }
 }
 
-// out[i] = factor * sum over parts of part[s][i], four elements a thread: A's dk, 4 parts, 80 MB in 14 us
+// One or two arrays (blockIdx.y) of `count` elements: out[i] = factor * sum over parts of part[s][i], four elements a thread;
+// a part holds the arrays one behind the other.  A's dk and dv, 4 parts: 160 MB in XX us.
+template <typename T> struct Sums { T* out[2]; float factor[2]; };
+
 template <typename E>
-__global__ __launch_bounds__(256) void xa_sum_kernel(const float* part, long stride, int parts, long count, float factor,
-                                                     typename E::raw* out) {
-    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(256) void xa_sum_kernel(const float* part, int parts, long count, Sums<typename E::raw> to) {
+    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4, stride = gridDim.y * count;
     if (i >= count) return;
+    part += blockIdx.y * count + i;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int s = 0; s < parts; ++s) {
-        const float4 v = *reinterpret_cast<const float4*>(part + s * stride + i);
+        const float4 v = *reinterpret_cast<const float4*>(part + s * stride);
         a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
+    const float factor = to.factor[blockIdx.y];
     uint2 u;
     u.x = E::pair(a.x * factor, a.y * factor);
     u.y = E::pair(a.z * factor, a.w * factor);
-    *reinterpret_cast<uint2*>(out + i) = u;
+    *reinterpret_cast<uint2*>(to.out[blockIdx.y] + i) = u;
 }
 
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
@@ -852,7 +864,7 @@ Plan plan_of(int B, long R, int Lk, int Hk, int D) {
     const long keys = (Lk + kKeys - 1) / kKeys, rows = (R + kStep - 1) / kStep;
     n.fwd = parts_for(n.row_groups, keys, (n.dp <= 64 ? 4 : 2) * kCus, 6.0);
     n.dq = parts_for(n.row_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, 6.0);
-    n.dkv = parts_for(n.key_groups, rows, (n.dp <= 64 ? 3 : 1) * kCus, 6.0);
+    n.dkv = parts_for(n.key_groups, rows, (n.dp <= 64 ? 3 : n.dp <= 96 ? 2 : 1) * kCus, 6.0);
     return n;
 }
 
@@ -873,10 +885,10 @@ bool near_rows(const Att& p) {
 template <typename E, int DP> int launch_fwd(Att p, const Plan& n, hipStream_t st) {
     p.splits = n.fwd;
     const long blocks = n.row_groups * n.fwd, rows = (long)p.B * p.Hk * p.R;
-    if (bad_grid(blocks) || bad_grid((rows + 3) / 4)) return -3;
+    if (bad_grid(blocks) || (n.fwd > 1 && bad_grid(rows))) return -3;
     const auto kernel = near_keys(p) ? xa_fwd_kernel<E, DP, true> : xa_fwd_kernel<E, DP, false>;
     kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.rtiles);
-    if (n.fwd > 1) xa_join_kernel<E, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, rows);
+    if (n.fwd > 1) xa_join_kernel<E, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, (unsigned)rows);
     return DP_LAUNCH_STATUS();
 }
 
@@ -891,14 +903,12 @@ template <typename E, int DP> int launch_bwd(Att p, const Plan& n, hipStream_t s
     const auto dkv = near_rows(p) ? xa_dkv_kernel<E, DP, true> : xa_dkv_kernel<E, DP, false>;
     dq<<<dim3((unsigned)(n.row_groups * n.dq)), 256, 0, st>>>(p, n.rtiles);
     if (n.dq > 1)
-        xa_sum_kernel<E><<<dim3((unsigned)((qn + 1023) / 1024)), 256, 0, st>>>(p.part, qn, n.dq, qn, p.scale, (T*)p.dq);
+        xa_sum_kernel<E><<<dim3((unsigned)((qn + 1023) / 1024)), 256, 0, st>>>(p.part, n.dq, qn, {{(T*)p.dq, nullptr}, {p.scale, 1.f}});
     p.splits = n.dkv;
     dkv<<<dim3((unsigned)(n.key_groups * n.dkv)), 256, 0, st>>>(p, n.ktiles);
-    if (n.dkv > 1) {
-        const dim3 g((unsigned)((kv + 1023) / 1024));
-        xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part, 2 * kv, n.dkv, kv, p.scale, (T*)p.dk);
-        xa_sum_kernel<E><<<g, 256, 0, st>>>(p.part + kv, 2 * kv, n.dkv, kv, 1.f, (T*)p.dv);
-    }
+    if (n.dkv > 1)
+        xa_sum_kernel<E><<<dim3((unsigned)((kv + 1023) / 1024), 2), 256, 0, st>>>(p.part, n.dkv, kv,
+                                                                                   {{(T*)p.dk, (T*)p.dv}, {p.scale, 1.f}});
     return DP_LAUNCH_STATUS();
 }
 
