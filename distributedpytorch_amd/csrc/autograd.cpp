@@ -45,7 +45,11 @@ const void* in(const Tensor& t) { return t.defined() ? t.const_data_ptr() : null
 void* out(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 Tensor some(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
-void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+// (what a launch needs of a tensor that no Python check has seen: the operators are reachable as torch.ops.dpamd)
+void* stream(const Tensor& t) {
+    TORCH_CHECK(dp.gn_fwd != nullptr && t.is_cuda(), "dpamd operators take GPU tensors, after ops._backend.native()");
+    return c10::hip::getCurrentHIPStream(t.get_device()).stream();
+}
 
 int type_code(const Tensor& t) {
     switch (t.scalar_type()) {

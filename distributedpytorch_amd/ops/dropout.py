@@ -103,7 +103,8 @@ def dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, seed: Option
     ``int`` is used as it is (its low 64 bits); an int64 tensor of one element on ``x``'s device is read when the kernel
     runs, so a captured graph draws a new mask when the program has written a new seed between replays — it must hold
     the same value when backward runs.  ``x`` may be contiguous or channels-last (the mask follows memory order); other
-    layouts are copied.  GPU types: bf16, fp16, fp32."""
+    layouts are copied.  A call that is run again for its backward pass (activation checkpointing) needs a ``seed`` of its
+    own: a drawn one would be another.  GPU types: bf16, fp16, fp32."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout: p must lie in [0, 1], got {p}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):

@@ -219,3 +219,53 @@ def test_one_tensor_as_every_operand():
     (gx,) = torch.autograd.grad(y, x, x.detach())
     ga, gr = torch.autograd.grad(ya, (a, r), x.detach())
     assert torch.equal(gx, ga + gr)
+
+
+def _calls():
+    """(inputs by name, call) of each operator, every input wanting a gradient."""
+    from distributedpytorch_amd import ops
+    x, r = (_rand(2, 24, 9, 11, seed=s).contiguous(memory_format=torch.channels_last) for s in (1, 2))
+    w, b = _rand(24, seed=3, dtype=torch.float32), _rand(24, seed=4, dtype=torch.bfloat16)
+    q, k, v = _rand(2, 70, 4, 40, seed=5), _rand(2, 90, 2, 40, seed=6), _rand(2, 90, 2, 40, seed=7)
+    return {
+        "norm": (dict(x=x, weight=w, bias=b, residual=r), lambda x, weight, bias, residual:
+                 ops.group_norm_act(x, 6, weight, bias, act="silu", residual=residual)),
+        "norm without act": (dict(x=x, weight=w, bias=b, residual=r), lambda x, weight, bias, residual:
+                             ops.group_norm_act(x, 6, weight, bias, residual=residual)),
+        "dropout": (dict(x=x, residual=r), lambda x, residual: ops.dropout(x, 0.4, seed=9, residual=residual)),
+        "attention": (dict(q=q, k=k, v=v), ops.cross_attention),
+    }
+
+
+@pytest.mark.parametrize("name", ["norm", "norm without act", "dropout", "attention"])
+def test_each_input_alone_gets_the_gradient_it_gets_among_all(name):
+    inputs, call = _calls()[name]
+    leaves = {n: t.clone().requires_grad_(True) for n, t in inputs.items()}
+    y = call(**leaves)
+    dy = _rand(*y.shape, seed=11)
+    want = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)))
+    again = torch.autograd.grad(y, list(leaves.values()), dy)               # the same graph a second time
+    for n, g in zip(leaves, again):
+        assert torch.equal(g, want[n]) and g.dtype == leaves[n].dtype and g.shape == leaves[n].shape
+    for n in inputs:
+        one = {m: t.clone().requires_grad_(m == n) for m, t in inputs.items()}
+        out = call(**one)
+        assert torch.equal(out, y)
+        (g,) = torch.autograd.grad(out, one[n], dy)
+        assert torch.equal(g, want[n])
+    with torch.inference_mode():
+        assert torch.equal(call(**inputs), y)
+
+
+@pytest.mark.parametrize("name", ["norm", "dropout", "attention"])
+def test_checkpointed_calls_give_the_same_gradients(name):
+    from torch.utils.checkpoint import checkpoint
+    inputs, call = _calls()[name]
+    leaves = {n: t.clone().requires_grad_(True) for n, t in inputs.items()}
+    y = call(**leaves)
+    dy = _rand(*y.shape, seed=11)
+    want = torch.autograd.grad(y, list(leaves.values()), dy)
+    again = checkpoint(lambda *a: call(*a), *leaves.values(), use_reentrant=False)
+    assert torch.equal(again, y)
+    for g, w in zip(torch.autograd.grad(again, list(leaves.values()), dy), want):
+        assert torch.equal(g, w)
