@@ -170,15 +170,15 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     return v;
 }
 
-// A team of `wide` waves (1 or 4, whole in one block of N threads) takes one (image, group): its items are the group's
-// (row range, channel) pairs, in memory order.
+// A team of 16, 64 or 256 threads, whole in one block of N, takes one (image, group): its items are the group's (row range,
+// channel) pairs, in memory order.
 struct Team { long gi, n; int c0, items, first, step; bool on; };
 
-template <int N> __device__ __forceinline__ Team team_of(const Geo& g, long groups, int wide, long block) {
+template <int N> __device__ __forceinline__ Team team_of(const Geo& g, long groups, int team, long block) {
     const int tid = threadIdx.x;
     Team t;
-    t.step = wide * 64;
-    t.gi = block * (N / 64 / wide) + tid / t.step;
+    t.step = team;
+    t.gi = block * (N / team) + tid / team;
     t.on = t.gi < groups;
     t.n = t.on ? t.gi / g.G : 0;
     t.c0 = t.on ? (int)(t.gi % g.G) * g.cpg : 0;
@@ -187,9 +187,11 @@ template <int N> __device__ __forceinline__ Team team_of(const Geo& g, long grou
     return t;
 }
 
-__device__ __forceinline__ double team_sum(double v, int wide, double* lds) {
-    v = wave_sum_d(v);
-    if (wide == 1) return v;
+__device__ __forceinline__ double team_sum(double v, int team, double* lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        if (o < team) v += __shfl_xor(v, o, 64);
+    if (team <= 64) return v;
     const int w = threadIdx.x >> 6;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[w] = v;
@@ -200,10 +202,10 @@ __device__ __forceinline__ double team_sum(double v, int wide, double* lds) {
 
 // stats[n, g] = (mean, rstd).  Every item is a sample with a mean and squared deviations of its own; all the terms that
 // join them are positive.
-__global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int wide, const float* __restrict__ part,
+__global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int team, const float* __restrict__ part,
                                                         const float* __restrict__ pivot, double* __restrict__ stats) {
     __shared__ double lds[4];
-    const Team t = team_of<256>(g, groups, wide, blockIdx.x);
+    const Team t = team_of<256>(g, groups, team, blockIdx.x);
     const float* base = part + t.n * g.splits * 2 * g.C + t.c0;
     const float* pv = pivot + t.n * g.C + t.c0;
     double sm = 0.0;
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int 
         sm += (double)rows * (double)pv[c] + (double)base[(long)s * 2 * g.C + c];
     }
     const double count = (double)g.hw * g.cpg;
-    const double mean = team_sum(sm, wide, lds) / count;
+    const double mean = team_sum(sm, team, lds) / count;
     double m2 = 0.0;
 #pragma unroll 4
     for (int i = t.first; i < t.items; i += t.step) {
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int 
         const double own = s2 - s1 * s1 / rows, d = (double)pv[c] + s1 / rows - mean;
         m2 += (own < 0.0 ? 0.0 : own) + d * d * rows;                                   // (a NaN stays one)
     }
-    m2 = team_sum(m2, wide, lds);
+    m2 = team_sum(m2, team, lds);
     if (t.on && t.first == 0) {
         stats[2 * t.gi] = mean;
         stats[2 * t.gi + 1] = 1.0 / sqrt(m2 / count + (double)g.eps);
@@ -380,14 +382,14 @@ __global__ __launch_bounds__(256) void gn_bwd_reduce_kernel(Geo g, const T* __re
 // parts a block.
 constexpr int kJoin = 1024;
 
-__global__ __launch_bounds__(kJoin) void gn_bwd_join_kernel(Geo g, long groups, int wide, int mean_blocks, long lines,
+__global__ __launch_bounds__(kJoin) void gn_bwd_join_kernel(Geo g, long groups, int team, int mean_blocks, long lines,
                                                             const float* __restrict__ part, const float* __restrict__ w,
                                                             float* __restrict__ means, float* __restrict__ dw,
                                                             float* __restrict__ db) {
     __shared__ double lds[2][kJoin];
     const int tid = threadIdx.x;
     if ((int)blockIdx.x < mean_blocks) {
-        const Team t = team_of<kJoin>(g, groups, wide, blockIdx.x);
+        const Team t = team_of<kJoin>(g, groups, team, blockIdx.x);
         const float* base = part + t.n * g.splits * 2 * g.C + t.c0;
         double a = 0.0, q = 0.0;
 #pragma unroll 4
@@ -397,8 +399,8 @@ __global__ __launch_bounds__(kJoin) void gn_bwd_join_kernel(Geo g, long groups, 
             a += wc * (double)base[(long)s * 2 * g.C + c];
             q += wc * (double)base[(long)s * 2 * g.C + g.C + c];
         }
-        a = team_sum(a, wide, lds[0]);
-        q = team_sum(q, wide, lds[1]);
+        a = team_sum(a, team, lds[0]);
+        q = team_sum(q, team, lds[1]);
         if (t.on && t.first == 0) {
             const double inv = 1.0 / ((double)g.hw * g.cpg);
             means[2 * t.gi] = (float)(a * inv);
@@ -478,16 +480,20 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
 }
 
 // ------------------------------------------------------------------------------------------------ groups that fit a block
-// Where a group's map fits the registers of one block (at most held(RES) packs for each of its 512 threads), the block
-// reads it once, takes the statistics from its registers (the mean first, then the squared differences from it) and writes
-// the result: one launch forward, two backward, and no second read.  Needs whole packs inside a group (cpg a multiple of
-// V).  A group's rows are pieces of cpg elements, often less than a cache line: the groups that share lines run next to
-// each other on one XCD, whose L2 then reads each line once (counted: 67 MB of a 67 MB map).  512 channels of 16 x 64 x 64
-// in 32 groups, bf16, ReLU, against the passes above: forward 38 us (51; 76 without that order) with inputs in the last
-// level of cache and 50 (62) without, backward 72 (78) and 88 (79).  A CU holds one block, so loads, sums and stores of a
-// block follow one another; two blocks (128 registers) took 58 us forward without cached inputs, 1,024 threads spilled.
+// Where a group's map fits the registers of one block (at most held<V>(RES) packs or elements for each of its 512 threads),
+// the block reads it once, takes the statistics from its registers (the mean first, then the squared differences from it) and
+// writes the result: one launch forward, two backward, and no second read.  A group's rows are pieces of cpg elements, often
+// less than a cache line: the groups that share lines run next to each other on one XCD, whose L2 then reads each line once
+// (counted: 67 MB of a 67 MB map).  512 channels of 16 x 64 x 64 in 32 groups, bf16, ReLU, against the passes above: forward
+// 38 us (51; 76 without that order) with inputs in the last level of cache and 50 (62) without, backward 72 (78) and 88 (79).
+// A CU holds one block, so loads, sums and stores of a block follow one another; two blocks (128 registers) took 58 us
+// forward without cached inputs, 1,024 threads spilled.
 constexpr int kBlock = 512;
-constexpr int held(bool res) { return res ? 8 : 16; }        // (a residual is one more operand to hold)
+// Packs (a residual is one more operand) or single elements that a thread holds.  Single ones serve groups that split packs
+// and rows off 16 bytes, up to 8,192 elements a group, in pieces of a few bytes, which one block reads in less time than
+// three launches take: 3 x 48 channels of 2,720 positions, fp32, 16 groups, forward and backward 24 us (34 in passes); 32
+// images of them 52 (54); 16 elements a thread, since 40 (20,480 a group) took 70 us where the passes take 49.
+template <int V> constexpr int held(bool res) { return V == 1 ? 16 : res ? 8 : 16; }
 
 __device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned total) {
     const unsigned x = id & 7, i = id >> 3, q = total >> 3, r = total & 7;
@@ -532,7 +538,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_fwd_kernel(Geo g, const T* __r
                                                              const float* __restrict__ w, const float* __restrict__ b,
                                                              T* __restrict__ y, double* __restrict__ stats) {
     constexpr bool kExact = sizeof(T) == 4;
-    constexpr int K = held(RES);
+    constexpr int K = held<V>(RES);
     __shared__ double lds[kBlock / 64];
     const long id = xcd_order(blockIdx.x, gridDim.x);
     const Slab s = slab_of(g, id);
@@ -592,7 +598,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
                                                              const double* __restrict__ stats, T* __restrict__ dx,
                                                              T* __restrict__ dres, float* __restrict__ part) {
     constexpr bool kExact = sizeof(T) == 4, kAct = ACT != kNone;
-    constexpr int K = held(RES);
+    constexpr int K = held<V>(RES);
     __shared__ float lds[2 * V * kBlock];
     __shared__ double sums[kBlock / 64];
     const long id = xcd_order(blockIdx.x, gridDim.x);
@@ -666,8 +672,11 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
     }
 }
 
-bool fits_slab(const Geo& g, int V, bool res) {
-    return V > 1 && g.cpg % V == 0 && g.cpg / V <= kBlock && g.hw <= (long)held(res) * (kBlock / (g.cpg / V));
+// At most two blocks for each of the 256 CUs, one after the other: a block takes 4 us forward and 10 backward however little
+// it holds.  64 x 512 x 7 x 7, bf16, ReLU, forward and backward: 64 groups 235 us against 41 in passes, 32 groups 118 against
+// 39; 16 images, 64 groups 65 against 39.
+template <int V> bool fits_slab(const Geo& g, long groups, bool res) {
+    return groups <= 512 && g.cpg % V == 0 && g.cpg / V <= kBlock && g.hw <= (long)held<V>(res) * (kBlock / (g.cpg / V));
 }
 
 Geo make_slab(Geo g, int V) {
@@ -695,11 +704,10 @@ Geo make_geo(long images, long hw, int C, int G, int V, float eps, long ldx, lon
     return g;
 }
 
-// waves of a team: four where a group has more than a wave's worth of items
-int team_width(const Geo& g) { return (long)g.cpg * g.splits > 64 ? 4 : 1; }
+// threads of a team, by the group's items: 16,384 groups of two items take 7 us with 16 threads each, 17 with 64
+int team_of_group(const Geo& g) { const long items = (long)g.cpg * g.splits; return items > 64 ? 256 : items > 16 ? 64 : 16; }
 
-// blocks of `waves` waves for all teams
-long team_blocks(long groups, int wide, int waves) { return (groups * wide + waves - 1) / waves; }
+long team_blocks(long groups, int team, int threads) { return (groups * team + threads - 1) / threads; }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -721,22 +729,23 @@ struct Fwd {
     hipStream_t stream;
 };
 
+template <typename T, int V, int ACT, bool RES> int run_slab_fwd(const Geo& g, long groups, const Fwd& f) {
+    gn_slab_fwd_kernel<T, V, ACT, RES><<<dim3((unsigned)groups), kBlock, 0, f.stream>>>(
+        make_slab(g, V), (const T*)f.x, (const T*)f.res, f.w, f.b, (T*)f.y, f.stats);
+    return DP_LAUNCH_STATUS();
+}
+
 template <typename T, int V, int ACT, bool RES>
 int run_fwd(const Geo& g, long images, const Fwd& f) {
     const long blocks = images * g.cblocks * g.splits, groups = images * g.G;
-    const int wide = team_width(g);
+    const int team = team_of_group(g);
     if (blocks > 0x7fffffffL || groups > 0x7fffffffL) return -3;
-    if constexpr (V > 1) {
-        if (fits_slab(g, V, RES)) {
-            gn_slab_fwd_kernel<T, V, ACT, RES><<<dim3((unsigned)groups), kBlock, 0, f.stream>>>(
-                make_slab(g, V), (const T*)f.x, (const T*)f.res, f.w, f.b, (T*)f.y, f.stats);
-            return DP_LAUNCH_STATUS();
-        }
-    }
+    if (fits_slab<V>(g, groups, RES)) return run_slab_fwd<T, V, ACT, RES>(g, groups, f);
+    if (g.cpg % V && fits_slab<1>(g, groups, RES)) return run_slab_fwd<T, 1, ACT, RES>(g, groups, f);
     float* pivot = f.ws;
     float* part = f.ws + images * g.C;
     gn_stats_kernel<T, V><<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, part, pivot);
-    gn_finish_kernel<<<dim3((unsigned)team_blocks(groups, wide, 4)), 256, 0, f.stream>>>(g, groups, wide, part, pivot, f.stats);
+    gn_finish_kernel<<<dim3((unsigned)team_blocks(groups, team, 256)), 256, 0, f.stream>>>(g, groups, team, part, pivot, f.stats);
     const auto apply = g.cpg % V == 0 ? gn_apply_kernel<T, V, 1, ACT, RES> : gn_apply_kernel<T, V, V, ACT, RES>;
     apply<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(g, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, (T*)f.y);
     return DP_LAUNCH_STATUS();
@@ -747,20 +756,25 @@ struct Bwd {
     hipStream_t stream;
 };
 
+// blocks for dw and db
+unsigned sum_blocks(const Geo& g, const Bwd& f) { return f.dw || f.db ? (unsigned)(((long)g.C + 15) / 16) : 0; }
+
+template <typename T, int V, int ACT, bool RES> int run_slab_bwd(const Geo& g, long images, const Bwd& f) {
+    gn_slab_bwd_kernel<T, V, ACT, RES><<<dim3((unsigned)(images * g.G)), kBlock, 0, f.stream>>>(
+        make_slab(g, V), (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, (T*)f.dx, (T*)f.dres, f.ws);
+    const unsigned sums = sum_blocks(g, f);
+    if (sums) gn_bwd_join_kernel<<<dim3(sums), kJoin, 0, f.stream>>>(g, 0, 64, 0, images, f.ws, f.w, nullptr, f.dw, f.db);
+    return DP_LAUNCH_STATUS();
+}
+
 template <typename T, int V, int ACT, bool RES>
 int run_bwd(const Geo& g, long images, const Bwd& f) {
     const long blocks = images * g.cblocks * g.splits, groups = images * g.G;
-    const int wide = team_width(g);
-    const unsigned sums = f.dw || f.db ? (unsigned)(((long)g.C + 15) / 16) : 0;
+    const int team = team_of_group(g);
+    const unsigned sums = sum_blocks(g, f);
     if (blocks > 0x7fffffffL || groups > 0x7fffffffL) return -3;
-    if constexpr (V > 1) {
-        if (fits_slab(g, V, RES)) {
-            gn_slab_bwd_kernel<T, V, ACT, RES><<<dim3((unsigned)groups), kBlock, 0, f.stream>>>(
-                make_slab(g, V), (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, (T*)f.dx, (T*)f.dres, f.ws);
-            if (sums) gn_bwd_join_kernel<<<dim3(sums), kJoin, 0, f.stream>>>(g, 0, 1, 0, images, f.ws, f.w, nullptr, f.dw, f.db);
-            return DP_LAUNCH_STATUS();
-        }
-    }
+    if (fits_slab<V>(g, groups, RES)) return run_slab_bwd<T, V, ACT, RES>(g, images, f);
+    if (g.cpg % V && fits_slab<1>(g, groups, RES)) return run_slab_bwd<T, 1, ACT, RES>(g, images, f);
     float* means = f.ws;
     float* part = f.ws + 2 * images * g.G;
     const bool one = g.cpg % V == 0;
@@ -768,8 +782,8 @@ int run_bwd(const Geo& g, long images, const Bwd& f) {
     const auto apply = one ? gn_bwd_apply_kernel<T, V, 1, ACT, RES> : gn_bwd_apply_kernel<T, V, V, ACT, RES>;
     reduce<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, part);
-    const unsigned mean_blocks = (unsigned)team_blocks(groups, wide, kJoin / 64);
-    gn_bwd_join_kernel<<<dim3(mean_blocks + sums), kJoin, 0, f.stream>>>(g, groups, wide, (int)mean_blocks, images * g.splits,
+    const unsigned mean_blocks = (unsigned)team_blocks(groups, team, kJoin);
+    gn_bwd_join_kernel<<<dim3(mean_blocks + sums), kJoin, 0, f.stream>>>(g, groups, team, (int)mean_blocks, images * g.splits,
                                                                         part, f.w, means, f.dw, f.db);
     apply<<<dim3((unsigned)blocks), 256, 0, f.stream>>>(
         g, (const T*)f.dy, (const T*)f.x, (const T*)f.res, f.w, f.b, f.stats, means, (T*)f.dx, (T*)f.dres);

@@ -114,6 +114,17 @@ def test_group_norm_shapes(shape, groups, dtype):
     _check_norm(shape, groups, dtype, "silu", False, seed=sum(shape))
 
 
+@pytest.mark.parametrize("shape,groups", [
+    # on both sides of what one block holds: single elements, packs, and more blocks than two a CU
+    ((3, 48, 51, 53), 16), ((3, 48, 55, 51), 16), ((2, 64, 61, 33), 8), ((2, 64, 65, 67), 8), ((16, 96, 9, 7), 32),
+    ((17, 96, 9, 7), 32), ((17, 192, 9, 7), 32),
+])
+@pytest.mark.parametrize("act,residual", [("relu", False), ("silu", True), (None, True)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_group_norm_groups_in_one_block_and_in_passes(shape, groups, act, residual, dtype):
+    _check_norm(shape, groups, dtype, act, residual, seed=sum(shape))
+
+
 @pytest.mark.parametrize("layout", ["contiguous", "slice", "odd slice"])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_group_norm_layouts(layout, dtype):
