@@ -368,7 +368,7 @@ __device__ __forceinline__ Work work_of(const Att& p, int tiles) {
     return w;
 }
 
-// Where part s of `blocks` begins (at most 2^23 blocks and 64 parts: the product fits 32 bits, whose division is a tenth of
+// Where part s of `blocks` begins (at most 2^23 blocks and 256 parts: the product fits 32 bits, whose division is a tenth of
 // a 64-bit one's instructions).
 __device__ __forceinline__ int part_of(int blocks, int s, int parts) { return (int)((unsigned)blocks * (unsigned)s / (unsigned)parts); }
 
@@ -499,33 +499,53 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void xa_fwd_kernel(Att p, in
         }
 }
 
-// joins the splits of one row: a wave per row, its parts' statistics in one access and its sums in the next: 6.6 us for 64
-// rows of 17 parts, 21 us for 33,800 rows of 5 parts of 128 columns (88 MB: 4.2 TB/s)
-template <typename E, int DP>
+// Joins the parts of one row: W waves a row, each its range of at most 64 parts, whose statistics it reads in one access and
+// whose sums in the next.  One wave for up to 16 parts (33,800 rows of 5 parts of 128 columns: 21 us, 88 MB at 4.2 TB/s), four
+// for more.
+template <typename E, int DP, int W>
 __global__ __launch_bounds__(256) void xa_join_kernel(Att p, unsigned rows) {
     typedef typename E::raw T;
-    const unsigned id = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (id >= rows) return;
+    __shared__ float ms[4], ls[4], as[4][DP];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned id = blockIdx.x * (4 / W) + wave / W;
+    if (id >= rows) return;                          // (W = 4: a block is a row)
     const unsigned bh = id / (unsigned)p.R, r = id - bh * (unsigned)p.R;
-    const float* base = p.part + ((long)bh * p.splits * p.R + r) * (DP + 2);
+    const int per = (p.splits + W - 1) / W, first = wave % W * per;
+    const int mine = p.splits - first < per ? p.splits - first : per;
     const long step = (long)p.R * (DP + 2);
-    // lane s weighs part s (at most 64 parts)
-    const float own = lane < p.splits ? base[lane * step + DP] : -kInf, sum = lane < p.splits ? base[lane * step + DP + 1] : 0.f;
+    const float* base = p.part + ((long)bh * p.splits * p.R + r) * (DP + 2) + first * step;
+    // lane s weighs part s
+    const float own = lane < mine ? base[lane * step + DP] : -kInf, sum = lane < mine ? base[lane * step + DP + 1] : 0.f;
     float m = own;
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, k, 64));
     const float f = m == -kInf ? 0.f : __builtin_amdgcn_exp2f((own - m) * p.c);
-    const float l = wave_sum(sum * f);
+    float l = wave_sum(sum * f);
     float a0 = 0.f, a1 = 0.f;
     const int d = lane * 2;
 #pragma unroll 8
-    for (int s = 0; s < p.splits; ++s) {
+    for (int s = 0; s < mine; ++s) {
         const float g = __shfl(f, s, 64);
         if (d < DP) {
             const float2 o = *reinterpret_cast<const float2*>(base + s * step + d);
             a0 = fmaf(o.x, g, a0);
             a1 = fmaf(o.y, g, a1);
+        }
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) { ms[wave] = m; ls[wave] = l; }
+        if (d < DP) { as[wave][d] = a0; as[wave][d + 1] = a1; }
+        __syncthreads();
+        if (wave) return;
+        m = ms[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) m = __builtin_elementwise_maximum(m, ms[w]);
+        l = a0 = a1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float g = m == -kInf ? 0.f : __builtin_amdgcn_exp2f((ms[w] - m) * p.c);
+            l = fmaf(ls[w], g, l);
+            if (d < DP) { a0 = fmaf(as[w][d], g, a0); a1 = fmaf(as[w][d + 1], g, a1); }
         }
     }
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
@@ -838,10 +858,10 @@ __global__ __launch_bounds__(256) void xa_sum_kernel(const float* part, int part
 
 int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 
-// Parts of a long axis: `groups` workgroups of `steps` blocks each run in rounds of `slots` workgroups, so the time goes
-// with rounds / parts; each part more costs the join about `extra` blocks' time, and none is shorter than four blocks.
-int parts_for(long groups, long steps, long slots, double extra) {
-    const long most = (steps + 3) / 4 < 64 ? (steps + 3) / 4 : 64;
+// Parts of a long axis, at most `most` and of two blocks at least: `groups` workgroups of `steps` blocks each run in rounds of
+// `slots` workgroups, so the time goes with rounds / parts; each part more costs the join the time of about `extra` blocks.
+int parts_for(long groups, long steps, long slots, double extra, long most) {
+    if ((steps + 1) / 2 < most) most = (steps + 1) / 2;
     int best = 1;
     double least = 1e300;
     for (long n = 1; n <= most; ++n) {
@@ -865,9 +885,11 @@ Plan plan_of(int B, long R, int Lk, int Hk, int D) {
     n.key_groups = (long)B * Hk * n.ktiles;
     // workgroups that a CU holds: registers for heads of 96 and more, LDS and registers for the rest
     const long keys = (Lk + kKeys - 1) / kKeys, rows = (R + kStep - 1) / kStep;
-    n.fwd = parts_for(n.row_groups, keys, (n.dp <= 64 ? 4 : 2) * kCus, 6.0);
-    n.dq = parts_for(n.row_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, 6.0);
-    n.dkv = parts_for(n.key_groups, rows, (n.dp <= 64 ? 3 : n.dp <= 96 ? 2 : 1) * kCus, 6.0);
+    // (what a join costs goes with the rows or keys that a tile really has)
+    const double rowjoin = 6.0 * (double)(R < kRows ? R : kRows) / kRows, keyjoin = 6.0 * (double)(Lk < kRows ? Lk : kRows) / kRows;
+    n.fwd = parts_for(n.row_groups, keys, (n.dp <= 64 ? 4 : 2) * kCus, rowjoin, 256);
+    n.dq = parts_for(n.row_groups, keys, (n.dp <= 64 ? 3 : 2) * kCus, rowjoin, 64);
+    n.dkv = parts_for(n.key_groups, rows, (n.dp <= 64 ? 3 : n.dp <= 96 ? 2 : 1) * kCus, keyjoin, 64);
     return n;
 }
 
@@ -891,7 +913,8 @@ template <typename E, int DP> int launch_fwd(Att p, const Plan& n, hipStream_t s
     if (bad_grid(blocks) || (n.fwd > 1 && bad_grid(rows))) return -3;
     const auto kernel = near_keys(p) ? xa_fwd_kernel<E, DP, true> : xa_fwd_kernel<E, DP, false>;
     kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(p, n.rtiles);
-    if (n.fwd > 1) xa_join_kernel<E, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, (unsigned)rows);
+    if (n.fwd > 16) xa_join_kernel<E, DP, 4><<<dim3((unsigned)rows), 256, 0, st>>>(p, (unsigned)rows);
+    else if (n.fwd > 1) xa_join_kernel<E, DP, 1><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(p, (unsigned)rows);
     return DP_LAUNCH_STATUS();
 }
 
