@@ -844,10 +844,13 @@ __global__ __launch_bounds__(256) void xa_sum_kernel(const float* part, int part
     if (i >= count) return;
     part += blockIdx.y * count + i;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
-        const float4 v = *reinterpret_cast<const float4*>(part + s * stride);
-        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    for (int s = 0; s < parts; s += 8) {             // eight parts' loads in flight
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            v[k] = s + k < parts ? *reinterpret_cast<const float4*>(part + (s + k) * stride) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { a.x += v[k].x; a.y += v[k].y; a.z += v[k].z; a.w += v[k].w; }
     }
     const float factor = to.factor[blockIdx.y];
     uint2 u;

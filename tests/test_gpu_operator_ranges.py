@@ -269,3 +269,13 @@ def test_checkpointed_calls_give_the_same_gradients(name):
     assert torch.equal(again, y)
     for g, w in zip(torch.autograd.grad(again, list(leaves.values()), dy), want):
         assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("shape", [(1, 3, 20001, 1, 1, 64), (1, 1, 16641, 4, 1, 128), (2, 5, 2500, 2, 2, 40)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_cross_attention_of_few_rows_in_many_parts(shape, ragged):
+    """Up to 157 parts, joined by four waves; ragged: most parts hold no key."""
+    b, lk = shape[0], shape[2]
+    lens = torch.tensor([lk // 3, 0][:b], dtype=torch.int64, device="cuda") if ragged else None
+    mask = torch.arange(lk, device="cuda").remainder(130).ge(65).expand(b, lk) if ragged else None
+    _check(*_inputs(*shape, torch.bfloat16, seed=lk), lens=lens, mask=mask)
