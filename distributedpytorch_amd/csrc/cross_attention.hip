@@ -898,7 +898,7 @@ Plan plan_of(int B, long R, int Lk, int Hk, int D) {
 
 bool bad(int B, int Lq, int Lk, int Hk, int share, int D) {
     return B <= 0 || Lq <= 0 || Lk <= 0 || Hk <= 0 || share <= 0 || D <= 0 || D % 8 || D > 128 ||
-           (long)Lq * share > (1L << 29) || (long)B * Hk * share > 0x7fffffffL || Lk > 0x7fffff00;
+           (long)Lq * share > (1L << 29) || (long)B * Hk * share > 0x7fffffffL || Lk > (1 << 29);
 }
 
 bool bad_grid(long n) { return n <= 0 || n > 0x7fffffffL; }
