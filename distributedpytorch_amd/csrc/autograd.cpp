@@ -4,7 +4,8 @@
 // Python object that the forward thread touched last is a cache miss: as Python nodes, a forward and backward pass of
 // dropout on 1 x 256 x 33 x 33 took 77 us and of an fp32 group norm on 3 x 48 x 65 x 97 (46 us of kernels) 136 us of host
 // time, where a node that only returns its gradient takes 38 us, nearly all of it the change of threads.  Here they take
-// what that change and the launches take.
+// 27 to 54 and 60 to 99, by where the two threads run: dropout's backward 38 us where torch.relu's takes 38, group norm's 46
+// with the gradient of x alone and 58 with those of weight and bias.
 //
 // Arguments are checked in Python (ops/group_norm.py, ops/dropout.py, ops/cross_attention.py).  What is here: layouts that
 // the kernels read, outputs, workspaces, launches on the tensors' GPU and its current stream.
