@@ -709,6 +709,10 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void xa_dkv_kernel(Att p, in
     bool on = key < len;
     if (on && p.mask) on = p.mask[(long)w.b * p.mask_ld + key] != 0;
     const bool wave_on = __any(on);
+    // (here, where every lane of the wave takes part: a lane counts one key of the image, whichever keys the wave holds)
+    KeySets sets(p, w.b, len);
+    sets.ahead(0);
+    const bool lone = len > 0 && len <= 64 && __popcll(sets.of(0)) == 1;
     const long bh = (long)w.b * p.Hk + w.hk;
     const int nst = (p.R + kStep - 1) / kStep;
     const int st0 = part_of(nst, w.split, p.splits);
@@ -801,9 +805,6 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void xa_dkv_kernel(Att p, in
         if (st + 1 < st1) block(Q1, D1, S1, Q0, D0, S0, st + 1);
     }
     if (key >= p.Lk) return;
-    KeySets sets(p, w.b, len);
-    sets.ahead(0);
-    const bool lone = len > 0 && len <= 64 && __popcll(sets.of(0)) == 1;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) {
         if (!on) dv[t] = zero16();

@@ -1,0 +1,54 @@
+"""Cross attention whose masks leave a few keys of a short sequence, or one key of a long one (csrc/cross_attention.hip).
+
+Tolerances: those of tests/test_gpu_cross_attention.py."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from test_gpu_cross_attention import _check, _inputs  # noqa: E402
+pytestmark = pytest.mark.gpu
+
+
+def _gradients(q, k, v, dout, lens=None, mask=None):
+    from distributedpytorch_amd import ops
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    return torch.autograd.grad(ops.cross_attention(*leaves, key_lengths=lens, key_mask=mask), leaves, dout)
+
+
+def _keys(lk, *on):
+    m = torch.zeros(lk, dtype=torch.bool)
+    m[list(on)] = True
+    return m
+
+
+def _without(lk, *off):
+    return ~_keys(lk, *off)
+
+
+@pytest.mark.parametrize("mask", [
+    _keys(40, 20, 35), _without(33, 0), _keys(33, 31, 32), _keys(33, 1, 2, 32), _keys(48, 15, 16, 40), _keys(63, 30, 62),
+    _keys(64, 0, 63), _keys(64, 31, 32), _without(64, 32), _keys(63, 33, 34), _keys(40, 3, 4), _keys(17, 2, 16),
+], ids=lambda m: f"{m.sum()} of {len(m)}")
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_key_that_takes_part_in_one_block_gets_its_gradient(mask, dtype):
+    lk = len(mask)
+    q, k, v, dout = _inputs(2, 3, lk, 4, 2, 64, dtype, seed=lk)
+    mask = mask.expand(2, lk).cuda()
+    _check(q, k, v, dout, mask=mask)
+    dk, dv = _gradients(q, k, v, dout, mask=mask)[1:]
+    assert (dk != 0).any(-1)[mask].all() and (dv != 0).any(-1)[mask].all()
+
+
+@pytest.mark.parametrize("lk", [33, 40, 47, 63, 64, 100])
+@pytest.mark.parametrize("density", [0.1, 0.5, 0.9])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_random_masks_with_lengths_of_one_block(lk, density, dim):
+    q, k, v, dout = _inputs(12, 3, lk, 2, 1, dim, torch.float16, seed=lk)
+    g = torch.Generator().manual_seed(dim)
+    mask = (torch.rand(12, lk, generator=g) < density).cuda()
+    lens = torch.randint(0, min(lk, 64) + 1, (12,), generator=g).cuda()
+    _check(q, k, v, dout, mask=mask)
+    _check(q, k, v, dout, lens=lens, mask=mask)
