@@ -183,6 +183,25 @@ __device__ __forceinline__ int key_count(const Att& p, int b) {
     return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
 }
 
+// Whether a single key of the image's first len takes part: P = 1 whatever its score, dq = dk = 0.  Asked by whole waves, and
+// only by those that saw one key themselves.
+__device__ __forceinline__ bool single_key(const Att& p, int b, int len) {
+    if (!p.mask) return len == 1;
+    const unsigned char* mask = p.mask + (long)b * p.mask_ld;
+    int n = 0;
+    for (int k = 0; k < len && n < 2; k += 512) {
+        bool on[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = k + j * 64 + (int)(threadIdx.x & 63);
+            on[j] = key < len && mask[key] != 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n += __popcll(__ballot(on[j]));
+    }
+    return n == 1;
+}
+
 // offset of row r of key head hk in a tensor of rows
 __device__ __forceinline__ int position(const Att& p, int r) { return p.share == 1 ? r : (int)((unsigned)r / (unsigned)p.share); }
 
@@ -558,8 +577,8 @@ __global__ __launch_bounds__(256) void xa_join_kernel(Att p, unsigned rows) {
 
 // ------------------------------------------------------------------------------------------------ backward
 // dq of 128 rows, and delta for xa_dkv.  delta = rowsum(do o) comes from the rounded o; over a few keys o is as large as
-// v and that rounding would show in dS = P (dP - delta), so an image whose keys fit one block takes
-// delta = sum_j P_j dP_j from its registers instead.
+// v and that rounding would show in dS = P (dP - delta), so an image whose keys lie within one block (its length: a mask may
+// leave as few of a longer one) takes delta = sum_j P_j dP_j from its registers instead.
 template <typename E, int DP, bool DMA>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int tiles) {
     typedef typename E::raw T;
@@ -605,6 +624,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
     KeyStream<T, DP, DMA> ks_(p, p.k, p.vk, w.b, w.hk), vs_(p, p.v, p.vv, w.b, w.hk);
     KeySets sets(p, w.b, len);
     unsigned long long set = 0, next = 0;
+    int seen = 0;                                       // keys that take part
     if (kb0 < kb1) {
         sets.ahead(kb0);
         next = sets.of(kb0);
@@ -618,6 +638,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
             vs_.put(vt);
         }
         set = next;
+        seen += __popcll(set);
         arrive();
         if (kb + 1 < kb1) {
             next = sets.of(kb + 1);
@@ -653,7 +674,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
             }
             del = halves_sum(sum);
             if (row_on && h == 0) p.delta[bh * p.R + r] = -del;
-            if (__popcll(set) == 1) return;             // a single key: P = 1 whatever the score, dq = dk = 0
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -670,6 +690,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
     for (int kb = kb0; kb < kb1; kb += 2) {
         block(K0, V0, K1, V1, kb);
         if (kb + 1 < kb1) block(K1, V1, K0, V0, kb + 1);
+    }
+    if (seen == 1 && single_key(p, w.b, len)) {
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
     }
     if (!row_on) return;
     const long at = dense_row(p, w.b, w.hk, r);
@@ -709,10 +733,8 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void xa_dkv_kernel(Att p, in
     bool on = key < len;
     if (on && p.mask) on = p.mask[(long)w.b * p.mask_ld + key] != 0;
     const bool wave_on = __any(on);
-    // (here, where every lane of the wave takes part: a lane counts one key of the image, whichever keys the wave holds)
-    KeySets sets(p, w.b, len);
-    sets.ahead(0);
-    const bool lone = len > 0 && len <= 64 && __popcll(sets.of(0)) == 1;
+    // (here, where every lane of the wave takes part; a key is on two lanes)
+    const bool lone = __popcll(__ballot(on)) == 2 && single_key(p, w.b, len);
     const long bh = (long)w.b * p.Hk + w.hk;
     const int nst = (p.R + kStep - 1) / kStep;
     const int st0 = part_of(nst, w.split, p.splits);

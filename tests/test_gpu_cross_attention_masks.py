@@ -52,3 +52,24 @@ def test_random_masks_with_lengths_of_one_block(lk, density, dim):
     lens = torch.randint(0, min(lk, 64) + 1, (12,), generator=g).cuda()
     _check(q, k, v, dout, mask=mask)
     _check(q, k, v, dout, lens=lens, mask=mask)
+
+
+@pytest.mark.parametrize("lq,lk,dim,at", [(50, 65, 64, (64, 0)), (1, 200, 128, (130, 199)), (33, 1023, 96, (1000, 3)),
+                                          (3, 1100, 32, (1024, 1099)), (2, 20001, 64, (20000, 12345)), (600, 2049, 64, (2048, 700))])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_single_key_of_a_long_sequence_has_no_score_gradient(lq, lk, dim, at, dtype):
+    """P = 1 whatever the score, however long the sequence is; image 2 has two keys, image 3 none."""
+    q, k, v, dout = _inputs(4, lq, lk, 4, 2, dim, dtype, seed=lk)
+    mask = torch.zeros(4, lk, dtype=torch.bool, device="cuda")
+    for i, j in ((0, at[0]), (1, at[1]), (2, at[0]), (2, at[1])):
+        mask[i, j] = True
+    _check(q, k, v, dout, mask=mask)
+    dq, dk, dv = _gradients(q, k, v, dout, mask=mask)
+    for i in (0, 1, 3):
+        assert not dq[i].any() and not dk[i].any()
+    assert (dq[2] != 0).any(-1).all() and (dk[2] != 0).any(-1)[mask[2]].all() and (dv != 0).any(-1)[mask].all()
+    # a length that leaves one of two unmasked keys
+    lens = torch.full((4,), max(at), dtype=torch.int32, device="cuda")
+    _check(q, k, v, dout, lens=lens, mask=mask)
+    dq, dk, dv = _gradients(q, k, v, dout, lens=lens, mask=mask)
+    assert not dq.any() and not dk.any() and (dv[2] != 0).any(-1).sum() == dv.shape[2]
