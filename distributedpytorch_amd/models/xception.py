@@ -213,6 +213,9 @@ class AlignedXception(nn.Module):
         for blk in chain:
             blk.input_sole = blk is not self.block2
         if mid != MID_CHANNELS:
+            for name, m in self.named_modules():
+                if name.startswith(_PADDED) and getattr(m, "num_features", None) == mid:
+                    m.stored_wider = True
             self._register_state_dict_hook(_logical_state_dict)
             self._register_load_state_dict_pre_hook(self._physical_state_dict)
             # Initialise as the 728-channel network does: the 768-wide layers drew kaiming_normal_ with their physical

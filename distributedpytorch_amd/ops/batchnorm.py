@@ -406,6 +406,7 @@ class BatchNorm2d(nn.Module):
     even in training mode (the reference's ``freeze_bn``)."""
 
     batch_statistics = True        # (ops.group_norm.GroupNorm2d, which can stand in its place, has none)
+    stored_wider = False           # its map holds zero channels that the architecture does not have (models.xception)
 
     def __init__(self, num_features: int, eps: float = 1e-5, momentum: float = 0.1,
                  sync: bool = False, frozen: bool = False, process_group=None):

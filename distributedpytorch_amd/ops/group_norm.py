@@ -103,7 +103,13 @@ class GroupNorm2d(nn.Module):
 def convert_group_norm(module: nn.Module, num_groups: int = 32) -> nn.Module:
     """``module`` with every ``BatchNorm2d`` replaced by a ``GroupNorm2d`` of the same weight and bias (in place; a module
     that is itself one is returned as its replacement), with the largest number of groups that divides both
-    ``num_groups`` and its channels.  A module used in two places stays one module."""
+    ``num_groups`` and its channels.  A module used in two places stays one module.  Layers that are stored wider than
+    the architecture has them (Xception's 728-channel flow where it is padded) are refused, and nothing is replaced:
+    a group's statistics would take in channels that do not exist."""
+    if any(getattr(m, "stored_wider", False) for m in module.modules()):
+        raise NotImplementedError("convert_group_norm: the module stores a BatchNorm2d wider than it is (Xception's 728 channels "
+                                  "as 768, models.xception): zero channels would enter a group's statistics; DPAMD_X65_PAD=0 "
+                                  "builds the model without them")
     return _convert(module, num_groups, {})
 
 
