@@ -123,8 +123,8 @@ class XceptionBlock(nn.Module):
         units = list(self.rep)
         # pre-activation quirk of the published weights: the shortcut sees the activated input
         if self.skip is not None:
-            if self.skipbn.training and not self.skipbn.frozen and self.skip.can_fuse_stats(x) \
-                    and self.skip.can_passthrough(x):
+            if self.skipbn.batch_statistics and self.skipbn.training and not self.skipbn.frozen \
+                    and self.skip.can_fuse_stats(x) and self.skip.can_passthrough(x):
                 # the shortcut convolution first, the units on its passthrough: the units' input gradient is added in
                 # the shortcut's data-gradient store loop (no add kernel)
                 sk, st, x = self.skip(x, with_stats=True, passthrough=True, sole_consumer=sole)

@@ -156,7 +156,7 @@ class _FoldedPointwise(torch.autograd.Function):
 def can_fold(sep, bn2, x: torch.Tensor) -> bool:
     dw, bn1, pw = sep.conv1, sep.bn, sep.pointwise
     return (_FOLD and B.use_hip(x) and x.dtype == torch.bfloat16 and torch.is_grad_enabled()
-            and bn1.training and not bn1.frozen
+            and bn1.batch_statistics and bn2.batch_statistics and bn1.training and not bn1.frozen
             and bn2.training and not bn2.frozen and 0.0 <= bn2.momentum < 1.0
             and dw.can_fuse_stats(x) and pw.bias is None and pw.groups == 1 and pw.kernel_size == (1, 1)
             and pw.stride == (1, 1) and pw.padding == (0, 0)
@@ -168,8 +168,8 @@ EVAL_FOLD = True          # (module switch for tests / tools)
 
 def _eval_fold_ok(sep, bn2, x: torch.Tensor) -> bool:
     pw = sep.pointwise
-    return (EVAL_FOLD and not bn2.training and not sep.bn.training and not torch.is_grad_enabled() and B.use_hip(x)
-            and x.dtype == torch.bfloat16 and pw.bias is None and pw.groups == 1 and pw.kernel_size == (1, 1)
+    return (EVAL_FOLD and sep.bn.batch_statistics and bn2.batch_statistics and not bn2.training
+            and not sep.bn.training and not torch.is_grad_enabled() and B.use_hip(x) and x.dtype == torch.bfloat16 and pw.bias is None and pw.groups == 1 and pw.kernel_size == (1, 1)
             and pw.stride == (1, 1) and pw.padding == (0, 0) and pw.in_channels % 8 == 0 and pw.out_channels % 8 == 0)
 
 
@@ -187,6 +187,9 @@ def eval_fold_constants(sep, bn2=None):
             return None
         bn2 = st["bn2"]
     pw, bn1 = sep.pointwise, sep.bn
+    if not bn1.batch_statistics:             # (folded once, and converted to group norm since)
+        sep.__dict__.pop("_eval_fold", None)
+        return None
     a1, a2 = bn1.eval_affine(), bn2.eval_affine()
     key = (pw.weight._version, bn1._affine_key, bn2._affine_key, sep.__dict__.get("_eval_fold_epoch", 0))
     dev = pw.weight.device
@@ -208,7 +211,7 @@ def sepconv_bn_act(sep, bn2, x: torch.Tensor, relu: bool = False, residual: Opti
                    dropout: float = 0.0, passthrough: bool = False, sole_consumer: bool = False):
     """``act(BN2(pointwise(BN1(depthwise(x)))) + residual)`` for a ``models.xception.SeparableConv2d`` ``sep``.
     Training on the GPU path with local (non-synchronised, non-frozen) statistics folds BN1 into the pointwise
-    weights; everything else runs the ordinary composition.
+    weights; everything else (a ``GroupNorm2d`` in either place too) runs the ordinary composition.
 
     ``passthrough=True`` returns ``(out, x')``: ``x'`` is ``x`` routed through the depthwise node — use it as the
     block's shortcut and its gradient is added inside the depthwise data-gradient kernel (no add kernel).
@@ -226,7 +229,8 @@ def sepconv_bn_act(sep, bn2, x: torch.Tensor, relu: bool = False, residual: Opti
         return (y, x) if passthrough else y
     pt = passthrough and dw.can_passthrough(x)
     if not can_fold(sep, bn2, x):
-        if bn2.training and not sep.bn.frozen and dw.can_fuse_stats(x) and (pt or sole_consumer) and sep.bn.training:
+        if (sep.bn.batch_statistics and sep.bn.training and not sep.bn.frozen and bn2.training and dw.can_fuse_stats(x)
+                and (pt or sole_consumer)):
             if pt:
                 z, st, skip = dw(x, with_stats=True, passthrough=True, sole_consumer=sole_consumer)
             else:
