@@ -1,4 +1,4 @@
-"""Group norm inside models on the GPU: Xception's separable units."""
+"""Group norm inside models on the GPU: Xception's separable units, and FCN and DANet."""
 import copy
 import os
 import sys
@@ -86,3 +86,35 @@ def test_xception_converted_after_an_evaluation_keeps_no_folded_constants():
     leaf = x.detach().requires_grad_(True)
     net(leaf)[0].float().square().mean().backward()
     assert all(torch.isfinite(p.grad).all() for p in net.parameters())
+
+
+@pytest.mark.parametrize("name,classes,channels,layers", [("fcn_resnet18", 21, 3, 22), ("danet_resnet50", 1, 4, 58)])
+def test_fcn_and_danet_with_group_norm(name, classes, channels, layers):
+    """Evaluation, which computes what training computes without dropout, against fp32 on the CPU: every layer rounds its
+    weights, the convolution's map and the norm's, each by at most 2^-8 (spread 2^-8 / sqrt(3)) with random sign; four times the
+    spread of their sum.  Then steps of the training engine, eager and captured."""
+    from distributedpytorch_amd.models import build_model
+    from distributedpytorch_amd.ops import SoftmaxCrossEntropy
+    from distributedpytorch_amd.parallel import TrainEngine
+    from distributedpytorch_amd.utils import SegmentationMultiLosses
+    torch.manual_seed(0)
+    ref = build_model(name, classes, in_channels=channels, norm="group").eval()
+    x = torch.randn(2, channels, 97, 97, generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        want = ref(x)
+        got = copy.deepcopy(ref).cuda()(x.cuda().to(torch.bfloat16).contiguous(memory_format=torch.channels_last))
+    for a, b in zip(*(t if isinstance(t, tuple) else (t,) for t in (got, want))):
+        assert _rel(a, b) < 4 * (3 * layers / 3) ** 0.5 * HALF
+    y = torch.randint(0, 21, (2, 97, 97), dtype=torch.uint8) if classes > 1 else (torch.rand(2, 1, 97, 97) > 0.5).float()
+    for graph_step in (False, True):                       # (no learning: an untrained DANet's logits are in the hundreds)
+        crit = SoftmaxCrossEntropy(255) if classes > 1 else SegmentationMultiLosses(1)
+        eng = TrainEngine(copy.deepcopy(ref), crit, lr=0.0, momentum=0.0, weight_decay=0.0, device=torch.device("cuda", 0),
+                          graph_step=graph_step)
+        losses = [float(eng.train_step(x.cuda(), y.cuda())) for _ in range(6)]
+        assert all(v == v and v < float("inf") for v in losses) and len(eng._graphs) == int(graph_step), losses
+        if not graph_step:
+            eng.model.eval()
+            crit(eng.ddp(eng.prepare_input(x)), y.cuda()).backward()
+            still = [s.name for s in eng.ddp.arena.slots if not s.param.grad.any() or not torch.isfinite(s.param.grad).all()]
+            # (DANet's attention branches start with a gain of zero: their projections have no gradient yet)
+            assert all(".sa." in n and "_conv" in n for n in still), still
