@@ -70,6 +70,13 @@ void first_order(const char* what) {
     TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, ": no gradients of gradients (create_graph=True)");
 }
 
+// Nor do they carry a tangent along: one that came in would be missing from the result, without an error.
+void no_tangent(const char* what, std::initializer_list<Tensor> inputs) {
+    for (const Tensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, ": no forward-mode derivatives; set_backend('torch') "
+                                    "runs the plain formulation, which has them");
+}
+
 Tensor workspace(long floats, const Tensor& like) {
     return floats > 0 ? at::empty({floats}, like.options().dtype(at::kFloat)) : Tensor();
 }
@@ -154,6 +161,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 Tensor group_norm_act(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias,
                       const optional<Tensor>& residual, int64_t groups, double eps, int64_t act) {
     const Tensor w = some(weight), b = some(bias), r = some(residual);
+    no_tangent("group_norm_act", {x, w, b, r});
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b) || wanted(r)))
         return GroupNormAct::apply(x, weight, bias, residual, groups, eps, act);
     Tensor stats;
@@ -207,6 +215,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor dropout(const Tensor& x, const optional<Tensor>& residual, int64_t threshold, int64_t seed,
                const optional<Tensor>& device_seed, bool word) {
     const Tensor r = some(residual);
+    no_tangent("dropout", {x, r});
     if (at::GradMode::is_enabled() && (wanted(x) || wanted(r)))
         return Dropout::apply(x, residual, threshold, seed, device_seed, word);
     const Tensor d = dense(x);
@@ -280,6 +289,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 
 Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& lengths,
                        const optional<Tensor>& mask, double scale) {
+    no_tangent("cross_attention", {q, k, v});
     if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v)))
         return CrossAttention::apply(q, k, v, lengths, mask, scale);
     return attend(heads(q), heads(k), heads(v), some(lengths), some(mask), scale, nullptr);
