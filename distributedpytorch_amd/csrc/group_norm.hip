@@ -200,6 +200,12 @@ __device__ __forceinline__ double team_sum(double v, int team, double* lds) {
     return (own[0] + own[1]) + (own[2] + own[3]);
 }
 
+// 1 / std.  In a group of one element xhat is zero and dx = 0 whatever the element: with 1 / std = 0 both are, where the
+// difference of w dz and its mean, which is its rounding, times 1 / sqrt(eps) would not be.
+__device__ __forceinline__ double inv_std(const Geo& g, double var) {
+    return g.hw * g.cpg == 1 ? 0.0 : 1.0 / sqrt(var + (double)g.eps);
+}
+
 // stats[n, g] = (mean, rstd).  Every item is a sample with a mean and squared deviations of its own; all the terms that
 // join them are positive.
 __global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int team, const float* __restrict__ part,
@@ -229,7 +235,7 @@ __global__ __launch_bounds__(256) void gn_finish_kernel(Geo g, long groups, int 
     m2 = team_sum(m2, team, lds);
     if (t.on && t.first == 0) {
         stats[2 * t.gi] = mean;
-        stats[2 * t.gi + 1] = 1.0 / sqrt(m2 / count + (double)g.eps);
+        stats[2 * t.gi + 1] = inv_std(g, m2 / count);
     }
 }
 
@@ -470,9 +476,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
                      dz = act_bwd<ACT, kExact>(dz, z);
                  }
                  h[i] = dz;
-                 // w dz rounded by itself: in a group of one element it then equals m1 and the gradient is zero
-                 const float t = __fmul_rn(wc[i], dz) - m1[i % S];
-                 f[i] = nc.rs[i % S] * fmaf(-xd, k2[i % S], t);
+                 f[i] = nc.rs[i % S] * fmaf(-xd, k2[i % S], wc[i] * dz - m1[i % S]);
              }
              Pack<T, V>::store(ob + r * g.C, f);
              if constexpr (RES) Pack<T, V>::store(hb + r * g.C, h);
@@ -568,7 +572,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_fwd_kernel(Geo g, const T* __r
         if (s.on && s.row + (long)k * s.rows < g.hw)
 #pragma unroll
             for (int i = 0; i < V; ++i) { const float d = (a[k].get(i) - nc.mh[0]) - nc.ml[0]; sq = fmaf(d, d, sq); }
-    const double rstd = 1.0 / sqrt(block_sum((double)sq, lds) * inv + (double)g.eps);
+    const double rstd = inv_std(g, block_sum((double)sq, lds) * inv);
     if (threadIdx.x == 0) { stats[2 * id] = mean; stats[2 * id + 1] = rstd; }
     if (!s.on) return;
     nc.rstd[0] = rstd;
@@ -663,7 +667,7 @@ __global__ __launch_bounds__(kBlock) void gn_slab_bwd_kernel(Geo g, const T* __r
             for (int i = 0; i < V; ++i) {
                 const float xd = a[k].get(i) - mh;
                 h[i] = gradient(k, i, xd);
-                f[i] = rs * fmaf(-xd, k2, __fmul_rn(wc[i], h[i]) - m1);      // (as gn_bwd_apply_kernel)
+                f[i] = rs * fmaf(-xd, k2, wc[i] * h[i] - m1);
             }
             const long at = (s.n * g.hw + r) * g.C + (long)s.chunk * V;
             Pack<T, V>::store(dx + at, f);
