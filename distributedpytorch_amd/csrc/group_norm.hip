@@ -16,8 +16,9 @@
 //
 // Precision.  Statistics are sums of differences from a per-channel pivot (the mean of four spread positions), so a map
 // whose mean is far larger than its spread loses nothing to cancellation; channels are joined by their means and their
-// squared deviations (all terms positive) in 64 bits.  z is formed as x a + b with a and b split into a rounded value
-// and its remainder: its error is relative to z itself, so an activation's border falls where the definition puts it.
+// squared deviations (all terms positive) in 64 bits.  z is formed as x a + b, for ReLU with a and b split into a rounded value
+// and its remainder: its error is relative to z itself, so ReLU's border falls where the definition puts it (before a residual
+// is added: the sum's error is relative to the larger term).
 // No atomics: every sum has one order.
 #include "common.h"
 
@@ -489,7 +490,8 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(Geo g, const T* __res
 // writes the result: one launch forward, two backward, and no second read.  A group's rows are pieces of cpg elements, often
 // less than a cache line: the groups that share lines run next to each other on one XCD, whose L2 then reads each line once
 // (counted: 67 MB of a 67 MB map).  512 channels of 16 x 64 x 64 in 32 groups, bf16, ReLU, against the passes above: forward
-// 38 us (51; 76 without that order) with inputs in the last level of cache and 50 (62) without, backward 72 (78) and 88 (79).
+// 38 us (51; 76 without that order) with inputs in the last level of cache and 50 (62) without, backward 72 (78) and 84..88
+// (79).  Where inputs lie is not known here, and both directions together are faster in one block either way.
 // A CU holds one block, so loads, sums and stores of a block follow one another; two blocks (128 registers) took 58 us
 // forward without cached inputs, 1,024 threads spilled.
 constexpr int kBlock = 512;

@@ -51,7 +51,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     bool [B, Lk], True where a key takes part.  Keys that take no part may hold anything; a row without a key gives
     zeros and zero gradients.  ``scale``: positive, default ``1 / sqrt(D)``.  A channels-last map [N, C, H, W] is the
     sequence ``map.permute(0, 2, 3, 1).reshape(N, H * W, heads, C // heads)`` (a view).
-    GPU types: bf16, fp16; head widths up to 128."""
+    GPU types: bf16, fp16; head widths up to 128.  Scores, sums and statistics are held in 32 bits; probabilities, and the
+    gradients of scores, are rounded to the tensors' type before the product they enter."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("cross_attention: q [B, Lq, Hq, D], k and v [B, Lk, Hk, D], got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
