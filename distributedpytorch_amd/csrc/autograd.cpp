@@ -8,12 +8,16 @@
 // with the gradient of x alone and 58 with those of weight and bias.
 //
 // Arguments are checked in Python (ops/group_norm.py, ops/dropout.py, ops/cross_attention.py).  What is here: layouts that
-// the kernels read, outputs, workspaces, launches on the tensors' GPU and its current stream.
+// the kernels read, outputs, workspaces, launches on the tensors' GPU and its current stream.  The operators are reachable as
+// torch.ops.dpamd too, and hooks may put other tensors in a saved one's place: what a kernel would follow out of a tensor's
+// memory (another device, type or size) is refused here as well.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
+
+#include <climits>
 
 namespace {
 
@@ -46,7 +50,11 @@ const void* in(const Tensor& t) { return t.defined() ? t.const_data_ptr() : null
 void* out(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 Tensor some(const optional<Tensor>& t) { return t ? *t : Tensor(); }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
-// (what a launch needs of a tensor that no Python check has seen: the operators are reachable as torch.ops.dpamd)
+bool beside(const Tensor& t, const Tensor& x) { return !t.defined() || t.device() == x.device(); }
+bool like(const Tensor& t, const Tensor& x) {
+    return !t.defined() || (t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes());
+}
+
 void* stream(const Tensor& t) {
     TORCH_CHECK(dp.gn_fwd != nullptr && t.is_cuda(), "dpamd operators take GPU tensors, after ops._backend.native()");
     return c10::hip::getCurrentHIPStream(t.get_device()).stream();
@@ -82,6 +90,10 @@ Tensor workspace(long floats, const Tensor& like) {
 }
 
 // ------------------------------------------------------------------------------------------------ group norm
+bool channels(const Tensor& t, const Tensor& map) {
+    return !t.defined() || (t.device() == map.device() && t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == map.size(1));
+}
+
 // `t` where its memory is NHWC rows `ld` elements apart (a channels-last map or a channel slice of one), a channels-last
 // copy otherwise.
 Tensor rows(const Tensor& t, int64_t& ld) {
@@ -102,6 +114,8 @@ Tensor vector32(const Tensor& t) { return t.defined() ? t.to(at::kFloat).contigu
 
 Tensor norm_forward(const Tensor& map, const Tensor& w, const Tensor& b, const Tensor& residual, int64_t groups, double eps,
                     int64_t act, Tensor& stats) {
+    TORCH_CHECK(map.dim() == 4 && groups > 0 && map.size(1) <= INT_MAX && channels(w, map) && channels(b, map) && like(residual, map),
+                "group_norm_act: a [N, C, H, W] map, weight and bias [C], a residual like the map, all on one GPU");
     const c10::DeviceGuard guard(map.device());
     const Tensor y = map_like(map);
     stats = at::empty({map.size(0), groups, 2}, map.options().dtype(at::kDouble));
@@ -133,7 +147,10 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         first_order("group_norm_act");
         const auto saved = ctx->get_saved_variables();
         const auto plan = ctx->saved_data["plan"].toIntVector();
-        const Tensor &map = saved[0], &residual = saved[1], &w = saved[2], &b = saved[3], &stats = saved[4], &dy = grads[0];
+        const Tensor &map = saved[0], &residual = saved[1], &dy = grads[0];
+        const Tensor w = vector32(saved[2]), b = vector32(saved[3]), stats = saved[4].contiguous();
+        TORCH_CHECK(like(dy, map) && like(residual, map) && channels(w, map) && channels(b, map) && beside(stats, map),
+                    "group_norm_act: saved tensors and gradient belong on the map's GPU");
         const c10::DeviceGuard guard(map.device());
         const Tensor dx = map_like(map);
         Tensor dres = residual.defined() ? map_like(map) : Tensor(), dw, db;
@@ -182,6 +199,9 @@ Tensor ordered(const Tensor& t, at::IntArrayRef strides) {
 }
 
 Tensor drop(const Tensor& x, const Tensor& residual, int64_t threshold, int64_t seed, const Tensor& device_seed, bool word) {
+    TORCH_CHECK(like(residual, x) && beside(device_seed, x) &&
+                    (!device_seed.defined() || (device_seed.scalar_type() == at::kLong && device_seed.numel() == 1)),
+                "dropout: a residual like x, a seed of one int64 on x's GPU");
     const c10::DeviceGuard guard(x.device());
     const Tensor y = at::empty_strided(x.sizes(), x.strides(), x.options());
     if (x.numel())
@@ -241,10 +261,25 @@ struct Shape {
           D((int)q.size(3)) {}
 };
 
+// sizes that fit the launchers' ints, lengths and mask as the kernels read them
+void fits(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Tensor& mask) {
+    bool ok = q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(3) == q.size(3) &&
+              k.size(2) > 0 && q.size(2) % k.size(2) == 0 && k.scalar_type() == q.scalar_type() &&
+              v.scalar_type() == q.scalar_type() && beside(k, q) && beside(v, q) && beside(lengths, q) && beside(mask, q);
+    for (int i = 0; ok && i < 4; ++i) ok = q.size(i) <= 1 << 29 && k.size(i) <= 1 << 29;
+    if (ok && lengths.defined())
+        ok = lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == q.size(0) && lengths.is_contiguous();
+    if (ok && mask.defined())
+        ok = mask.scalar_type() == at::kBool && mask.dim() == 2 && mask.size(0) == q.size(0) && mask.size(1) == k.size(1) &&
+             (mask.stride(1) == 1 || mask.size(1) == 1);
+    TORCH_CHECK(ok, "cross_attention: q [B, Lq, Hq, D], k and v [B, Lk, Hk, D], int32 lengths [B], a bool mask [B, Lk], on one GPU");
+}
+
 long mask_stride(const Tensor& mask) { return mask.defined() ? mask.stride(0) : 0; }
 
 Tensor attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Tensor& mask, double scale,
               Tensor* lse) {
+    fits(q, k, v, lengths, mask);
     const c10::DeviceGuard guard(q.device());
     const Shape s(q, k);
     const Tensor o = at::empty(q.sizes(), q.options());
@@ -271,7 +306,11 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         first_order("cross_attention");
         const auto saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &n = saved[5], &m = saved[6];
+        const Tensor q = heads(saved[0]), k = heads(saved[1]), v = heads(saved[2]), o = heads(saved[3].contiguous()),
+                     lse = saved[4].contiguous(), &n = saved[5];
+        const Tensor m = saved[6].defined() && saved[6].stride(-1) != 1 ? saved[6].contiguous() : saved[6];
+        fits(q, k, v, n, m);
+        TORCH_CHECK(like(o, q) && like(grads[0], q) && beside(lse, q), "cross_attention: saved tensors and gradient belong on q's GPU");
         const c10::DeviceGuard guard(q.device());
         const Shape s(q, k);
         const Tensor d = heads(grads[0]);
