@@ -169,7 +169,8 @@ EVAL_FOLD = True          # (module switch for tests / tools)
 def _eval_fold_ok(sep, bn2, x: torch.Tensor) -> bool:
     pw = sep.pointwise
     return (EVAL_FOLD and sep.bn.batch_statistics and bn2.batch_statistics and not bn2.training
-            and not sep.bn.training and not torch.is_grad_enabled() and B.use_hip(x) and x.dtype == torch.bfloat16 and pw.bias is None and pw.groups == 1 and pw.kernel_size == (1, 1)
+            and not sep.bn.training and not torch.is_grad_enabled() and B.use_hip(x)
+            and x.dtype == torch.bfloat16 and pw.bias is None and pw.groups == 1 and pw.kernel_size == (1, 1)
             and pw.stride == (1, 1) and pw.padding == (0, 0) and pw.in_channels % 8 == 0 and pw.out_channels % 8 == 0)
 
 
