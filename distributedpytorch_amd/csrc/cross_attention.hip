@@ -183,8 +183,8 @@ __device__ __forceinline__ int key_count(const Att& p, int b) {
     return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
 }
 
-// Whether a single key of the image's first len takes part: P = 1 whatever its score, dq = dk = 0.  Asked by whole waves, and
-// only by those that saw one key themselves.
+// Whether a single key of the image's first len takes part: P = 1 whatever its score, so dS and with it dq and dk are zero (but
+// a NaN stays one: what the roundings left is multiplied by zero).  Asked by whole waves, and only by those that saw one key.
 __device__ __forceinline__ bool single_key(const Att& p, int b, int len) {
     if (!p.mask) return len == 1;
     const unsigned char* mask = p.mask + (long)b * p.mask_ld;
@@ -693,7 +693,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void xa_dq_kernel(Att p, int
     }
     if (seen == 1 && single_key(p, w.b, len)) {
 #pragma unroll
-        for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
+        for (int t = 0; t < DP / 32; ++t) acc[t] *= splat16(0.f);
     }
     if (!row_on) return;
     const long at = dense_row(p, w.b, w.hk, r);
@@ -829,8 +829,8 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void xa_dkv_kernel(Att p, in
     if (key >= p.Lk) return;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) {
-        if (!on) dv[t] = zero16();
-        if (!on || lone) dk[t] = zero16();
+        if (lone) dk[t] *= splat16(0.f);
+        if (!on) dk[t] = dv[t] = zero16();
     }
     const long at = (((long)w.b * p.Lk + key) * p.Hk + w.hk) * p.D;
     const long whole = (long)p.B * p.Lk * p.Hk * p.D;

@@ -73,3 +73,22 @@ def test_a_single_key_of_a_long_sequence_has_no_score_gradient(lq, lk, dim, at, 
     _check(q, k, v, dout, lens=lens, mask=mask)
     dq, dk, dv = _gradients(q, k, v, dout, lens=lens, mask=mask)
     assert not dq.any() and not dk.any() and (dv[2] != 0).any(-1).sum() == dv.shape[2]
+
+
+@pytest.mark.parametrize("lk,kind", [(1, "one key"), (60, "mask"), (60, "length"), (200, "mask"), (200, "length"), (5000, "mask")])
+def test_a_nan_query_reaches_the_gradients_of_a_single_key(lk, kind):
+    """P of that row is NaN, as its output is; the other rows' dq are zeros."""
+    from distributedpytorch_amd import ops
+    q, k, v, dout = _inputs(2, 40, lk, 4, 2, 64, torch.bfloat16, seed=lk)
+    q[0, 7, 3, 5] = float("nan")
+    lens = torch.ones(2, dtype=torch.int32, device="cuda") if kind == "length" else None
+    at = lk - 1 if kind == "mask" else 0
+    mask = _keys(lk, at).expand(2, lk).cuda() if kind == "mask" else None
+    out = ops.cross_attention(q, k, v, key_lengths=lens, key_mask=mask)
+    dq, dk, dv = _gradients(q, k, v, dout, lens, mask)
+    assert out[0, 7, 3].isnan().all() and dq[0, 7, 3].isnan().all()
+    assert dk[0, at, 1].isnan().all() and dv[0, at, 1].isnan().all()
+    for t, where in ((out, (0, 7, 3)), (dq, (0, 7, 3)), (dk, (0, at, 1)), (dv, (0, at, 1))):
+        t[where] = 0
+        assert not t.isnan().any()
+    assert not dq.any() and not dk.any()
